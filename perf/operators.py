@@ -1,4 +1,4 @@
-"""Cases for timing and comparing the operators of include/lcrc_ops.h.
+"""Cases for timing and comparing the operators that include/lcrc_pipeline.h declares.
 
 Two operators of a recogniser's output side, and the two of them as one small net:
 
