@@ -3,7 +3,9 @@
  *   - the rows SURVEY 8 marks "next": the mel-bank front-end on the GPU (f1), the posterior writer path (f2), the
  *     PhnDec decoder on the device (f3);
  *   - what a host that drives lists through several contexts per GPU uses (this repository's SpeechRec / phnrec CLI):
- *     zero-copy staging, buffers reserved ahead, device warm-up, launch order, decoder overlap, completion callback.
+ *     zero-copy staging, buffers reserved ahead, device warm-up, launch order, decoder overlap, completion callback;
+ *   - operators on matrices in device memory, for nets and scores of the caller's own: log probabilities, entropy and best
+ *     classes of rows of logits or posteriors; products of matrices held in 8-bit floating point.
  * Same library, same conventions as lcrc.h.  None of it is needed to put the library behind the reference's Traps.
  */
 #ifndef PHNREC_LCRC_PIPELINE_H
@@ -189,6 +191,83 @@ int lcrc_set_wait_mode(lcrc_ctx *ctx, int poll_interval_us);
  * fn = NULL switches it off.  Not called when a call launches nothing or fails before its launch. */
 typedef void (*lcrc_kernel_done_fn)(void *arg);
 int lcrc_set_kernel_done_callback(lcrc_ctx *ctx, lcrc_kernel_done_fn fn, void *arg);
+
+/* ---- operators on matrices in device memory ------------------------------------------------------
+ * No context: each call names the GPU it runs on, works on device pointers of that GPU, is queued on `hip_stream` (NULL =
+ * HIP's default stream) and returns without waiting for it.  The calling thread's current device is left as it was.  The
+ * library keeps nothing between calls and allocates nothing inside them: scratch memory is the caller's (`workspace`, its
+ * size from the function named beside it, aligned to 16 bytes), used from the call's start to the end of its work on the
+ * stream -- calls that may overlap on the device, captured graphs among them, need one each.  All calls may be captured.
+ * Errors: a negative code, text in lcrc_last_error(NULL).  Sizes of 0 rows are no-ops.  An argument structure is read
+ * during the call only.  Results do not depend on what else runs, and are the same in every run. */
+enum { LCRC_T_F32 = 0, LCRC_T_F16 = 1, LCRC_T_BF16 = 2, LCRC_T_E4M3 = 3 };
+
+/* Log probabilities of given classes, entropy and best classes of every row of a matrix x[rows][cols] (rows `ld` elements
+ * apart): the posteriors of this library's nets (LCRC_SCORE_PROBS; rows that do not add up to 1 are normalised) or any
+ * net's logits (LCRC_SCORE_LOGITS).  With l(c) = x(c) or ln x(c), and p(c) = exp(l(c)) / sum exp(l):
+ *   logp[r][j]              ln p of class labels[r][j]; 0 where the label is negative (no label), NaN where it is >= cols
+ *   entropy[r]              - sum p ln p, in nats, 0 ln 0 = 0
+ *   top_index / top_logp    the k classes with the largest x in falling order, equal values by rising index, and their ln p
+ * A class of p = 0 (logit -inf, posterior 0) has ln p = -inf and can be among the k best of a row that has no others.  In a
+ * row in which no class is left (all -inf; all 0) every ln p is -inf, the entropy 0 and the best are classes 0 .. k-1.  A
+ * NaN, a logit of +inf or a posterior that is negative or infinite makes the row's ln p and entropy NaN and its top_index -1.
+ * Sums in 32 bits.  Any output may be NULL. */
+enum { LCRC_SCORE_LOGITS = 0, LCRC_SCORE_PROBS = 1 };
+typedef struct lcrc_score_args {
+    const void *x;            /* [rows][cols]: LCRC_T_F32, LCRC_T_F16 or LCRC_T_BF16, aligned to its element             */
+    int type, form;           /* LCRC_T_*, LCRC_SCORE_*                                                                  */
+    int rows, cols;           /* cols 1 .. 2^30                                                                          */
+    long long ld;             /* elements from one row to the next, >= cols                                              */
+    const int *labels;        /* [rows][n_labels]                                                                        */
+    int n_labels, k;          /* 0 .. 64; 0 .. 64, <= cols                                                               */
+    float *logp;              /* [rows][n_labels]                                                                        */
+    float *entropy;           /* [rows]                                                                                  */
+    int *top_index;           /* [rows][k]                                                                               */
+    float *top_logp;          /* [rows][k]                                                                               */
+    void *workspace;
+    size_t workspace_bytes;
+} lcrc_score_args;
+size_t lcrc_score_workspace(int rows, int cols, int k);      /* 0: none needed */
+int lcrc_score(int device_id, const lcrc_score_args *args, void *hip_stream);
+
+/* Products of matrices held in 8-bit floating point.  The form: OCP e4m3 (largest value 448) in blocks of 128 consecutive
+ * columns of a row, each with its own scale 2^e, e the smallest integer >= -127 for which no finite value of the block
+ * exceeds 448 * 2^e (0 for a block of zeros); values are rounded to the nearest, ties to even.  Scales that are powers of
+ * two cost no accuracy beside a scale of any value (e4m3 keeps its 4 significant bits over 2^15) and are exact in every
+ * product.  NaN and infinities become NaN and do not count for the scale.  A matrix in this form is an opaque buffer of
+ * lcrc_fp8_bytes(rows, cols) bytes, aligned to 16, in the order the matrix instructions read it.
+ * lcrc_fp8_pack: src[rows][cols] (`ld` elements apart) of LCRC_T_F32 / F16 / BF16, or of LCRC_T_E4M3 with
+ * scales[rows][ceil(cols / 128)] (bytes, e + 127) as a checkpoint holds them; scales is NULL for the other types.
+ * lcrc_fp8_unpack: the values it stands for, as LCRC_T_F32 / F16 / BF16. */
+size_t lcrc_fp8_bytes(int rows, int cols);
+int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, long long ld, const unsigned char *scales,
+                  void *dst, void *hip_stream);
+int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *dst, int type, long long ld, void *hip_stream);
+
+/* y = act(x W^T + bias), x[rows][n_in] and W[n_out][n_in] (NeuralNet's layout, nn.cpp:702-740) in the 8-bit form: exact
+ * products of the held values, added up in 32 bits.  (Where y has 16 or 8 bits the matrix instructions cut off, inside each
+ * group of eight products, what lies 13 bits below the largest of them: at most 7 * 2^-13 of sum |x w|.)  x is a matrix in that form (LCRC_T_E4M3, ldx ignored) or is
+ * put into it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32, f16 or bf16
+ * rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
+ * LCRC_ACT_SIGMOID: 1 / (1 + exp(-v)); LCRC_ACT_FSIGMOID: the same with the reference's fast exponential (fexp.h:14-21),
+ * which its trained nets expect.  y overlaps no input. */
+enum { LCRC_ACT_NONE = 0, LCRC_ACT_SIGMOID = 1, LCRC_ACT_FSIGMOID = 2 };
+typedef struct lcrc_fp8_linear_args {
+    const void *x;
+    int x_type;               /* LCRC_T_*                                                                                */
+    int rows, n_in, n_out;
+    long long ldx;            /* elements from one row to the next, >= n_in                                              */
+    const void *w;            /* [n_out][n_in] in the 8-bit form                                                         */
+    const float *bias;        /* [n_out] or NULL                                                                         */
+    int act;                  /* LCRC_ACT_*                                                                              */
+    void *y;
+    int y_type;               /* LCRC_T_*                                                                                */
+    long long ldy;            /* elements from one row to the next, >= n_out                                             */
+    void *workspace;
+    size_t workspace_bytes;
+} lcrc_fp8_linear_args;
+size_t lcrc_fp8_linear_workspace(int rows, int n_in, int x_type);
+int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *args, void *hip_stream);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,7 @@ SYMBOLS = [
     "lcrc_output_configure", "lcrc_decoder_configure", "lcrc_set_posterior_readback", "lcrc_last_labels", "lcrc_set_decoder_overlap", "lcrc_prev_labels", "lcrc_set_launch_order",
     "lcrc_reset", "lcrc_push", "lcrc_delay",
     "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_kernel_name",
+    "lcrc_score_workspace", "lcrc_score", "lcrc_fp8_bytes", "lcrc_fp8_pack", "lcrc_fp8_unpack", "lcrc_fp8_linear_workspace", "lcrc_fp8_linear",
 ]
 
 LCRC_OK, LCRC_E_ARG, LCRC_E_IO, LCRC_E_MODEL, LCRC_E_DEVICE, LCRC_E_NOMEM, LCRC_E_UNSUPPORTED = \
@@ -53,6 +54,28 @@ class Frontend(C.Structure):
                 ("vector_step", C.c_int), ("nbanks_full", C.c_int), ("lower_freq", C.c_float),
                 ("higher_freq", C.c_float), ("preem_coef", C.c_float), ("scale", C.c_float),
                 ("dc_shift", C.c_float), ("z_mean_source", C.c_int), ("sent_mean_norm", C.c_int)]
+
+
+# element types of the operators on matrices in device memory, their forms and activations (include/lcrc_pipeline.h)
+T_F32, T_F16, T_BF16, T_E4M3 = 0, 1, 2, 3
+TYPES = {"f32": T_F32, "f16": T_F16, "bf16": T_BF16, "e4m3": T_E4M3}
+SCORE_FORMS = {"logits": 0, "probs": 1}
+ACTS = {"none": 0, "sigmoid": 1, "fsigmoid": 2}
+
+
+class ScoreArgs(C.Structure):
+    """struct lcrc_score_args (include/lcrc_pipeline.h); pointers are device addresses as ints, 0 / None = not wanted"""
+    _fields_ = [("x", C.c_void_p), ("type", C.c_int), ("form", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+                ("ld", C.c_longlong), ("labels", C.c_void_p), ("n_labels", C.c_int), ("k", C.c_int), ("logp", C.c_void_p),
+                ("entropy", C.c_void_p), ("top_index", C.c_void_p), ("top_logp", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Fp8LinearArgs(C.Structure):
+    """struct lcrc_fp8_linear_args (include/lcrc_pipeline.h)"""
+    _fields_ = [("x", C.c_void_p), ("x_type", C.c_int), ("rows", C.c_int), ("n_in", C.c_int), ("n_out", C.c_int),
+                ("ldx", C.c_longlong), ("w", C.c_void_p), ("bias", C.c_void_p), ("act", C.c_int), ("y", C.c_void_p),
+                ("y_type", C.c_int), ("ldy", C.c_longlong), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class LcrcError(RuntimeError):
@@ -159,6 +182,15 @@ def load():
     L.lcrc_debug_fail_alloc.argtypes = [C.c_int]
     L.lcrc_debug_fail_launch.argtypes = [C.c_int]
     L.lcrc_posteriors_rows.argtypes = [vp, _f32p, C.c_int, C.c_int, C.c_int, _f32p]
+    L.lcrc_score_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
+    L.lcrc_score.argtypes = [C.c_int, C.POINTER(ScoreArgs), vp]
+    L.lcrc_fp8_bytes.argtypes = [C.c_int, C.c_int]
+    L.lcrc_fp8_pack.argtypes = [C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_longlong, vp, vp, vp]
+    L.lcrc_fp8_unpack.argtypes = [C.c_int, vp, C.c_int, C.c_int, vp, C.c_int, C.c_longlong, vp]
+    L.lcrc_fp8_linear_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
+    L.lcrc_fp8_linear.argtypes = [C.c_int, C.POINTER(Fp8LinearArgs), vp]
+    for name in ("lcrc_score_workspace", "lcrc_fp8_bytes", "lcrc_fp8_linear_workspace"):
+        getattr(L, name).restype = C.c_size_t
     _lib = L
     return L
 
@@ -174,6 +206,47 @@ def device_ln(x, form, device=0):
     if rc != 0:
         raise LcrcError(rc, L.lcrc_last_error(None).decode())
     return y
+
+
+def _checked(rc):
+    if rc != 0:
+        raise LcrcError(rc, _lib.lcrc_last_error(None).decode())
+
+
+# -- operators on matrices in device memory: raw device pointers (ints), asynchronous on `stream` (int handle or None) --
+def score_workspace(rows, cols, k):
+    """bytes of scratch memory a score() of this size needs (lcrc_score_workspace)"""
+    return load().lcrc_score_workspace(rows, cols, k)
+
+
+def score(args, stream=None, device=0):
+    """ln p of given classes, entropy and the k best classes of rows of logits or posteriors; args: ScoreArgs (lcrc_score)"""
+    _checked(load().lcrc_score(device, args, stream))
+
+
+def fp8_bytes(rows, cols):
+    """bytes of a matrix [rows][cols] in the 8-bit form (lcrc_fp8_bytes)"""
+    return load().lcrc_fp8_bytes(rows, cols)
+
+
+def fp8_pack(src, type, rows, cols, ld, dst, scales=None, stream=None, device=0):
+    """rows of f32 / f16 / bf16, or of e4m3 with one exponent byte per block of 128 columns, into the 8-bit form (lcrc_fp8_pack)"""
+    _checked(load().lcrc_fp8_pack(device, src, type, rows, cols, ld, scales, dst, stream))
+
+
+def fp8_unpack(src, rows, cols, dst, type, ld, stream=None, device=0):
+    """the values a matrix in the 8-bit form stands for (lcrc_fp8_unpack)"""
+    _checked(load().lcrc_fp8_unpack(device, src, rows, cols, dst, type, ld, stream))
+
+
+def fp8_linear_workspace(rows, n_in, x_type):
+    """bytes of scratch memory an fp8_linear() of this size needs (lcrc_fp8_linear_workspace)"""
+    return load().lcrc_fp8_linear_workspace(rows, n_in, x_type)
+
+
+def fp8_linear(args, stream=None, device=0):
+    """y = act(x W^T + bias) with x and W in the 8-bit form; args: Fp8LinearArgs (lcrc_fp8_linear)"""
+    _checked(load().lcrc_fp8_linear(device, args, stream))
 
 
 def model_info(model_dir, nbanks):
