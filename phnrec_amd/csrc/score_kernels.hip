@@ -2,6 +2,13 @@
 // row of logits or posteriors.
 //     l(c) = x(c) or ln x(c);  m = max x (logits), 0 (posteriors);  e(c) = exp(x(c) - m) or x(c)
 //     S = sum e, T = sum e * (l - m);  ln p(c) = (l(c) - m) - ln S;  entropy = ln S - T / S
+// Every row is read once.  All accesses are 16 bytes wide: a row is cut into chunks of 16 bytes from its start, the last one
+// moved back so that it ends with the row (what it holds twice is masked), so any alignment of an element is served and
+// nothing outside the row is touched.
+//
+// NaN, +inf (and posteriors below 0) need no test for each value: they leave S at NaN or inf (a maximum skips NaN, but exp
+// carries it; inf - inf is NaN), a negative posterior shows in the rows' minimum.
+#include <algorithm>
 #include <cmath>
 
 #include "ops_dev.h"
@@ -10,107 +17,669 @@ namespace phnrec {
 
 namespace {
 
+typedef unsigned long long u64;
+
 constexpr int kThreads = 256;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLowest = -3.40282346638528859812e38f;
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
 
-// rising with the value, -0 and +0 alike; NaN never reaches it in a row whose result counts
+// W consecutive elements, 16 bytes where W is 16 / sizeof(X)
+template <typename X, int W>
+struct Chunk {
+    X v[W];
+    __device__ __forceinline__ float operator[](int i) const { return to_f32(v[i]); }
+};
+template <typename X, int W>
+__device__ __forceinline__ Chunk<X, W> load_chunk(const X *p)
+{
+    Chunk<X, W> c;
+    __builtin_memcpy(&c, p, sizeof(c));             // element-aligned: one unaligned 16-byte load
+    return c;
+}
+
+// ---- reductions ----
+// over the 16 lanes of a row of lanes; every lane gets the same bits (each step adds the same two numbers in both places)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)); }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v)
+{
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false), lo);
+}
+template <typename V, typename Op>
+__device__ __forceinline__ V reduce16(V v, Op op)
+{
+    v = op(v, dpp<0x128>(v));                       // row_ror:8, 4, 2, 1
+    v = op(v, dpp<0x124>(v));
+    v = op(v, dpp<0x122>(v));
+    return op(v, dpp<0x121>(v));
+}
+template <typename Op>
+__device__ __forceinline__ float reduce64(float v, Op op)
+{
+    v = reduce16(v, op);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return __builtin_elementwise_max(a, b); } };
+struct Min { __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); } };
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+
+// ---- a row's statistics ----
+struct Stats {
+    float m, S, T;      // S is NaN or inf in a row that is no distribution
+};
+
+// the sums over one value; m: the row's (or the running) maximum
+template <bool PROBS>
+__device__ __forceinline__ void add_value(float v, float m, float &S, float &T)
+{
+    if constexpr (PROBS) {
+        // v_log_f32 flushes what is below 2^-126: scaled by 2^32 there
+        const bool small = v < 0x1p-126f;
+        const float l = __builtin_amdgcn_logf(small ? v * 0x1p32f : v) - (small ? 32.0f : 0.0f);
+        S += v;
+        T += v > 0.0f ? v * l : 0.0f;               // (in units of ln 2: finish())
+    } else {
+        const float d = v - m;
+        const float e = __builtin_amdgcn_exp2f(d * kLog2e);
+        S += e;
+        T = fmaf(e, fmaxf(d, -1e30f), T);           // (0 * -inf)
+    }
+}
+template <bool PROBS>
+__device__ __forceinline__ float finish(float T) { return PROBS ? T * kLn2 : T; }
+
+struct Row {
+    float m, S, T, ln_s;
+    bool bad, none;
+    __device__ __forceinline__ Row(const Stats &s, bool negative)
+        : m(s.m), S(s.S), T(s.T), ln_s(logf(s.S)), bad(negative || !(s.S < INFINITY)), none(!(s.S > 0.0f)) {}
+    template <bool PROBS>
+    __device__ __forceinline__ float ln_p(float v) const
+    {
+        if (bad) return NAN;
+        if (none) return -INFINITY;
+        return (PROBS ? logf(v) : v - m) - ln_s;
+    }
+    __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - T / S; }
+};
+
+template <typename X, bool PROBS>
+__device__ __forceinline__ float label_score(const lcrc_score_args &a, const X *x, const Row &row, size_t at)
+{
+    const int c = a.labels[at];
+    return c < 0 ? 0.0f : c >= a.cols ? NAN : row.template ln_p<PROBS>(to_f32(x[c]));
+}
+__device__ __forceinline__ bool wants_top(const lcrc_score_args &a) { return a.k > 0 && (a.top_index || a.top_logp); }
+
+// ---- short rows: 16 lanes to a row ----
+// A value and its column as ONE double: the f32 value (its conversion leaves 29 bits free) and the column in the free bits,
+// complemented where that makes the lower column the larger number.  So one v_max_f64, a full-rate instruction, orders values
+// and columns together, and a lane keeps its K best by K maxima and K - 1 minima for each value.  -inf sits at -2^200, below
+// every f32; what is no class at all at -inf.
+__device__ __forceinline__ double pair_of(float v, int c)
+{
+    const double d = fmax((double)(v + 0.0f), -0x1p200);
+    const int hi = __double2hiint(d);
+    return __hiloint2double(hi, __double2loint(d) | ((c ^ ~(hi >> 31)) & 0x1fffffff));
+}
+__device__ __forceinline__ int column_of(double d)
+{
+    return (__double2loint(d) ^ ~(__double2hiint(d) >> 31)) & 0x1fffffff;
+}
+__device__ __forceinline__ float value_of(double d)
+{
+    return (float)__hiloint2double(__double2hiint(d), __double2loint(d) & ~0x1fffffff);
+}
+
+// J chunks of W values to a lane: up to 16 J W columns; K: the longest list of best classes.
+template <typename X, bool PROBS, int W, int J, int K>
+__global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_args a)
+{
+    const int lane = threadIdx.x & 15, cols = a.cols;
+    const size_t stride = (size_t)gridDim.x * (kThreads / 16);
+    for (size_t r = (size_t)blockIdx.x * (kThreads / 16) + threadIdx.x / 16; r < (size_t)a.rows; r += stride) {
+        const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        Chunk<X, W> raw[J];
+#pragma unroll
+        for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((16 * j + lane) * W, cols - W));
+        // (all chunks but the last J are whole)
+        const int last = (16 * (J - 1) + lane) * W, start = min(last, cols - W);
+        const auto live = [&](int j, int i) { return j < J - 1 || start + i >= last; };
+        const auto column = [&](int j, int i) { return (j < J - 1 ? (16 * j + lane) * W : start) + i; };
+        float m = kLowest, least = 0.0f;
+        Stats s = {0.0f, 0.0f, 0.0f};
+        if constexpr (!PROBS) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int i = 0; i < W; i++) m = fmaxf(m, raw[j][i]);       // (what is there twice does no harm)
+            s.m = m = reduce16(m, Max());
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                const float v = live(j, i) ? raw[j][i] : PROBS ? 0.0f : -INFINITY;
+                if constexpr (PROBS) least = fminf(least, v);
+                add_value<PROBS>(v, m, s.S, s.T);
+            }
+        s.S = reduce16(s.S, Add());
+        s.T = finish<PROBS>(reduce16(s.T, Add()));
+        if constexpr (PROBS) least = reduce16(least, Min());
+        const Row row(s, least < 0.0f);
+        if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
+        if (a.logp)
+            for (int j = lane; j < a.n_labels; j += 16) a.logp[r * a.n_labels + j] = label_score<X, PROBS>(a, x, row, r * a.n_labels + j);
+        if constexpr (K > 0) {
+            double best[K];
+#pragma unroll
+            for (int q = 0; q < K; q++) best[q] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int i = 0; i < W; i++) {
+                    double d = pair_of(raw[j][i], column(j, i));
+                    if (!live(j, i)) d = -INFINITY;
+#pragma unroll
+                    for (int q = 0; q < K; q++) {
+                        const double larger = fmax(best[q], d);
+                        d = fmin(best[q], d);
+                        best[q] = larger;
+                    }
+                }
+            double mine = 0.0;
+            for (int n = 0; n < a.k; n++) {                  // the best head of the 16 lists, taken off its list
+                const double top = reduce16(best[0], Max());
+                const bool won = best[0] == top;
+#pragma unroll
+                for (int q = 0; q < K; q++) best[q] = won ? (q + 1 < K ? best[q + 1] : -INFINITY) : best[q];
+                if (lane == n) mine = top;
+            }
+            if (lane < a.k) {
+                if (a.top_index) a.top_index[r * a.k + lane] = row.bad ? -1 : column_of(mine);
+                if (a.top_logp) a.top_logp[r * a.k + lane] = row.template ln_p<PROBS>(value_of(mine));
+            }
+        }
+    }
+}
+
+// ---- longer rows: the best classes by a threshold ----
+// A key orders values, then columns (or chunks, or positions): 32 bits that rise with the value, -0 and +0 alike, and the
+// complement of the column below them; 0 is below every key of a value.
 __device__ __forceinline__ unsigned ordered(float x)
 {
     const unsigned b = __float_as_uint(x + 0.0f);
     return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ unsigned long long make_key(float x, int c)
+__device__ __forceinline__ u64 make_key(float x, int c) { return ((u64)ordered(x) << 32) | (0xffffffffu - (unsigned)c); }
+__device__ __forceinline__ int key_column(u64 k) { return (int)(0xffffffffu - (unsigned)k); }
+__device__ __forceinline__ float key_value(u64 k)
 {
-    return ((unsigned long long)ordered(x) << 32) | (0xffffffffu - (unsigned)c);
+    const unsigned o = (unsigned)(k >> 32);
+    return __uint_as_float(o ^ (~(unsigned)((int)o >> 31) | 0x80000000u));
 }
 
-template <typename V, typename Op>
-__device__ __forceinline__ V block_reduce(V v, V *slot, Op op)
+// The k-th largest (1 <= k <= 64) of the 64 lanes' numbers, bit by bit from the top: a candidate stands if k lanes reach it.
+// One compare a bit on the vector side, the count on the scalar side.
+__device__ __forceinline__ unsigned kth_largest(unsigned v, int k, bool alive)
 {
-    for (int d = 32; d >= 1; d >>= 1) v = op(v, __shfl_xor(v, d));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = slot[0];
-    for (int w = 1; w < kThreads / 64; w++) v = op(v, slot[w]);
-    return v;
-}
-
-// One workgroup per row.
-template <typename X, bool PROBS>
-__global__ __launch_bounds__(kThreads) void score_kernel(const lcrc_score_args a)
-{
-    __shared__ float fslot[kThreads / 64];
-    __shared__ unsigned long long kslot[kThreads / 64];
-    const size_t r = blockIdx.x;
-    const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
-    const int tid = threadIdx.x, cols = a.cols;
-    const auto add = [](float p, float q) { return p + q; };
-
-    float m = -INFINITY;
-    bool bad = false;
-    for (int c = tid; c < cols; c += kThreads) {
-        const float v = to_f32(x[c]);
-        bad = bad || !(v < INFINITY) || (PROBS && !(v >= 0.0f));
-        m = fmaxf(m, v);
+    unsigned res = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const unsigned t = res | (1u << bit);
+        if (__popcll(__ballot(alive && v >= t)) >= k) res = t;
     }
-    bad = __syncthreads_or(bad);
-    m = PROBS ? 0.0f : block_reduce(m, fslot, [](float p, float q) { return fmaxf(p, q); });
-    float S = 0.0f, T = 0.0f;
-    if (m > -INFINITY)
-        for (int c = tid; c < cols; c += kThreads) {
-            const float v = to_f32(x[c]);
-            const float e = PROBS ? v : expf(v - m);
-            S += e;
-            if (e > 0.0f) T += e * (PROBS ? logf(v) : v - m);
-        }
-    S = block_reduce(S, fslot, add);
-    T = block_reduce(T, fslot, add);
-    const float ln_s = logf(S);
-    const auto ln_p = [&](float v) {
-        if (bad) return (float)NAN;
-        if (!(S > 0.0f)) return -INFINITY;
-        return (PROBS ? logf(v) : v - m) - ln_s;
+    return res;
+}
+__device__ __forceinline__ u64 kth_largest(u64 key, int k)
+{
+    const unsigned hi = (unsigned)(key >> 32), lo = (unsigned)key;
+    const unsigned h = kth_largest(hi, k, true);
+    const int more = __popcll(__ballot(hi > h));
+    unsigned l = 0;
+    if (__popcll(__ballot(hi >= h)) > k) l = kth_largest(lo, k - more, hi == h);
+    return ((u64)h << 32) | l;
+}
+
+constexpr int kCandidates = 512;       // candidates a team holds (more: the slow way)
+
+// A team of threads that works on one row: T threads, one wave or a whole workgroup.
+template <int T>
+struct Team {
+    static constexpr int kWaves = T / 64;
+    struct Shared {
+        u64 cand[kCandidates];
+        u64 best[T > 64 ? T : 1];
+        float slot[4 * kWaves];
+        u64 kslot[kWaves];
+        int count;
     };
-    if (a.entropy && tid == 0) a.entropy[r] = bad ? NAN : S > 0.0f ? ln_s - T / S : 0.0f;
-    if (a.logp && tid < a.n_labels) {
-        const int c = a.labels[r * a.n_labels + tid];
-        a.logp[r * a.n_labels + tid] = c < 0 ? 0.0f : c >= cols ? NAN : ln_p(to_f32(x[c]));
-    }
-    if (!a.top_index && !a.top_logp) return;
-    unsigned long long last = ~0ull;
-    for (int j = 0; j < a.k; j++) {
-        unsigned long long best = 0;
-        for (int c = tid; c < cols; c += kThreads) {
-            const unsigned long long key = make_key(to_f32(x[c]), c);
-            if (key < last && key > best) best = key;
-        }
-        last = block_reduce(best, kslot, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; });
-        if (tid == 0) {
-            const int c = (int)(0xffffffffu - (unsigned)last);
-            if (a.top_index) a.top_index[r * a.k + j] = bad ? -1 : c;
-            if (a.top_logp) a.top_logp[r * a.k + j] = bad ? NAN : ln_p(to_f32(x[c]));
+    Shared &sh;
+    const int t;
+    __device__ __forceinline__ Team(Shared &s) : sh(s), t(threadIdx.x % T) {}
+    __device__ __forceinline__ void sync() const
+    {
+        if constexpr (T > 64) __syncthreads();
+        else {                                                  // one wave: its LDS accesses are in order
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
     }
+    // the team's statistics from its threads': S and T move to the team's maximum
+    template <bool PROBS>
+    __device__ __forceinline__ Stats join(Stats s, float &least)
+    {
+        Stats all;
+        const auto moved = [](Stats &v, float m) {
+            if constexpr (!PROBS) {
+                const float d = fmaxf(v.m - m, -1e30f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+                v.T = f * fmaf(v.S, d, v.T);
+                v.S *= f;
+            }
+        };
+        all.m = PROBS ? 0.0f : reduce64(s.m, Max());
+        moved(s, all.m);
+        all.S = reduce64(s.S, Add());
+        all.T = reduce64(s.T, Add());
+        least = PROBS ? reduce64(least, Min()) : 0.0f;
+        if constexpr (T > 64) {
+            sync();
+            if ((t & 63) == 0) {
+                float *p = sh.slot + 4 * (t >> 6);
+                p[0] = all.m, p[1] = all.S, p[2] = all.T, p[3] = least;
+            }
+            sync();
+            float m = sh.slot[0];
+            for (int w = 1; w < kWaves; w++) m = fmaxf(m, sh.slot[4 * w]);
+            s = {m, 0.0f, 0.0f};
+            for (int w = 0; w < kWaves; w++) {
+                Stats v = {sh.slot[4 * w], sh.slot[4 * w + 1], sh.slot[4 * w + 2]};
+                moved(v, m);
+                s.S += v.S, s.T += v.T;
+                least = fminf(least, sh.slot[4 * w + 3]);
+            }
+            all = s;
+        }
+        return all;
+    }
+    __device__ __forceinline__ u64 max_key(u64 v)
+    {
+        for (int d = 32; d >= 1; d >>= 1) {
+            const u64 o = __shfl_xor(v, d);
+            v = o > v ? o : v;
+        }
+        if constexpr (T > 64) {
+            sync();
+            if ((t & 63) == 0) sh.kslot[t >> 6] = v;
+            sync();
+            for (int w = 0; w < kWaves; w++) v = sh.kslot[w] > v ? sh.kslot[w] : v;
+        }
+        return v;
+    }
+    // The k best of the team's keys, best first: out(rank, key), by the thread that finds it.
+    //   first          this thread's best (value, chunk) as a key, 0 if it has none
+    //   scan(f)        f(value, chunk, column) for all that this thread holds
+    // The threads are put into 64 groups.  The k-th best of the groups' bests is reached by at least k values, so the k best
+    // are among the values that reach it, and those lie with the k groups that do: only their threads look at their values
+    // again.  The few that remain are ranked by counting.  Rows made so that more remain than fit are done one rank after
+    // another.
+    template <typename Scan, typename Out>
+    __device__ __forceinline__ void top(int k, u64 first, const Scan &scan, const Out &out)
+    {
+        u64 group = first;
+        if constexpr (T > 64) {
+            sh.best[t] = first;
+            if (t == 0) sh.count = 0;
+            sync();
+            for (int w = 0; w < kWaves; w++) {
+                const u64 o = sh.best[64 * w + (t & 63)];
+                group = o > group ? o : group;
+            }
+        } else {
+            if (t == 0) sh.count = 0;
+            sync();
+        }
+        const u64 bar = kth_largest(group, k);
+        if (first >= bar && first != 0)
+            scan([&](float v, int chunk, int c) {
+                if (make_key(v, chunk) >= bar) {
+                    const int at = atomicAdd(&sh.count, 1);      // (any order: they are ranked by their keys)
+                    if (at < kCandidates) sh.cand[at] = make_key(v, c);
+                }
+            });
+        sync();
+        const int n = sh.count;
+        if (n <= kCandidates) {
+            for (int i = t; i < n; i += T) {
+                const u64 key = sh.cand[i];
+                int rank = 0;
+                for (int q = 0; q < n; q++) rank += sh.cand[q] > key ? 1 : 0;
+                if (rank < k) out(rank, key);
+            }
+        } else {
+            u64 last = ~0ull;
+            for (int q = 0; q < k; q++) {
+                u64 best = 0;
+                scan([&](float v, int, int c) {
+                    const u64 key = make_key(v, c);
+                    if (key < last && key > best) best = key;
+                });
+                last = max_key(best);
+                if (t == 0) out(q, last);
+            }
+        }
+        sync();                                                 // (the lists are free for the next row)
+    }
+};
+
+__device__ __forceinline__ void put_bad(const lcrc_score_args &a, size_t r, int rank)
+{
+    if (a.top_index) a.top_index[r * a.k + rank] = -1;
+    if (a.top_logp) a.top_logp[r * a.k + rank] = NAN;
+}
+template <bool PROBS>
+__device__ __forceinline__ void put_top(const lcrc_score_args &a, size_t r, const Row &row, int rank, u64 key)
+{
+    if (a.top_index) a.top_index[r * a.k + rank] = key_column(key);
+    if (a.top_logp) a.top_logp[r * a.k + rank] = row.template ln_p<PROBS>(key_value(key));
+}
+
+// ---- middle rows: a wave to a row, the row in its registers: J chunks of 16 bytes to a lane ----
+template <typename X, bool PROBS, int J>
+__global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_args a)
+{
+    constexpr int W = 16 / sizeof(X);
+    __shared__ typename Team<64>::Shared shared[kThreads / 64];
+    Team<64> team(shared[threadIdx.x >> 6]);
+    const int lane = team.t, cols = a.cols;
+    const size_t stride = (size_t)gridDim.x * (kThreads / 64);
+    for (size_t r = (size_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); r < (size_t)a.rows; r += stride) {
+        const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        Chunk<X, W> raw[J];
+#pragma unroll
+        for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((64 * j + lane) * W, cols - W));
+        const auto each = [&](const auto &f) {
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int at = (64 * j + lane) * W, start = min(at, cols - W);
+#pragma unroll
+                for (int i = 0; i < W; i++)
+                    if (start + i >= at) f(raw[j][i], 64 * j + lane, start + i);
+            }
+        };
+        float m = kLowest, least = 0.0f;
+        Stats s = {0.0f, 0.0f, 0.0f};
+        if constexpr (!PROBS) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int i = 0; i < W; i++) m = fmaxf(m, raw[j][i]);       // (what is there twice does no harm)
+            s.m = m = reduce64(m, Max());
+        }
+        each([&](float v, int, int) {
+            if constexpr (PROBS) least = fminf(least, v);
+            add_value<PROBS>(v, m, s.S, s.T);
+        });
+        s.S = reduce64(s.S, Add());
+        s.T = finish<PROBS>(reduce64(s.T, Add()));
+        if constexpr (PROBS) least = reduce64(least, Min());
+        const Row row(s, least < 0.0f);
+        if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
+        if (a.logp && lane < a.n_labels) a.logp[r * a.n_labels + lane] = label_score<X, PROBS>(a, x, row, r * a.n_labels + lane);
+        if (!wants_top(a)) continue;
+        if (row.bad) {
+            if (lane < a.k) put_bad(a, r, lane);
+            continue;
+        }
+        u64 first = 0;
+        each([&](float v, int chunk, int) {
+            const u64 key = make_key(v, chunk);
+            first = key > first ? key : first;
+        });
+        team.top(a.k, first, each, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
+    }
+}
+
+// ---- long rows: a workgroup to a row, or to a part of one ----
+struct Part {
+    int parts;                  // of a row
+    int chunks;                 // in a part
+    float4 *stats;              // [rows][parts]: m, S, T, the least value  (parts > 1)
+    u64 *keys;                  // [rows][parts][k], best first, 0 where a part has fewer
+};
+
+template <typename X, bool PROBS, int T>
+__global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, const Part p)
+{
+    constexpr int W = 16 / sizeof(X), U = 4;
+    __shared__ typename Team<T>::Shared shared;
+    Team<T> team(shared);
+    const int t = team.t, cols = a.cols, n_chunks = (cols + W - 1) / W;
+    const bool want_top = wants_top(a);
+    const size_t jobs = (size_t)a.rows * p.parts;
+    for (size_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const size_t r = job / p.parts;
+        const int from = (int)(job - r * p.parts) * p.chunks, to = min(from + p.chunks, n_chunks);
+        const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        Stats s = {kLowest, 0.0f, 0.0f};
+        float least = 0.0f, most = -INFINITY;
+        int most_at = -1;
+        for (int c0 = from + t; c0 < to; c0 += U * T) {
+            Chunk<X, W> raw[U];
+            bool whole[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) raw[u] = load_chunk<X, W>(x + min((c0 + u * T) * (long long)W, (long long)cols - W));
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + u * T;
+                whole[u] = c < to;
+                if (!whole[u]) continue;
+                float v = raw[u][W - 1];
+                const int twice = (int)max(0ll, (c + 1) * (long long)W - cols);       // of the row's last chunk
+#pragma unroll
+                for (int i = 0; i < W - 1; i++)
+                    if (i >= twice) v = fmaxf(v, raw[u][i]);
+                if (v > most || most_at < 0) {
+                    most = v;
+                    most_at = c;
+                }
+                top = fmaxf(top, v);
+            }
+            if constexpr (!PROBS)
+                if (top > s.m + 8.0f || (s.m == kLowest && top > s.m)) {     // the reference moves in steps: seldom
+                    const float d = fmaxf(s.m - top, -1e30f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+                    s.T = f * fmaf(s.S, d, s.T);
+                    s.S *= f;
+                    s.m = top;
+                }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (!whole[u]) continue;
+                const long long at = (c0 + u * T) * (long long)W;
+                if (at + W <= cols) {
+#pragma unroll
+                    for (int i = 0; i < W; i++) {
+                        if constexpr (PROBS) least = fminf(least, raw[u][i]);
+                        add_value<PROBS>(raw[u][i], s.m, s.S, s.T);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; i++)
+                        if (cols - W + i >= at) {
+                            if constexpr (PROBS) least = fminf(least, raw[u][i]);
+                            add_value<PROBS>(raw[u][i], s.m, s.S, s.T);
+                        }
+                }
+            }
+        }
+        s.T = finish<PROBS>(s.T);
+        s = team.template join<PROBS>(s, least);
+        const Row row(s, least < 0.0f);
+        if (p.parts == 1) {
+            if (a.entropy && t == 0) a.entropy[r] = row.entropy();
+            if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
+        } else if (t == 0) p.stats[job] = float4{s.m, s.S, s.T, least};
+        if (!want_top) continue;
+        if (row.bad) {
+            if (p.parts == 1 && t < a.k) put_bad(a, r, t);
+            continue;                               // (a bad part makes its row bad: its list is not read)
+        }
+        u64 *list = p.keys + job * a.k;
+        if (p.parts > 1) {
+            // a part with fewer values than k leaves zeros at its list's end
+            const long long here = min((long long)to * W, (long long)cols) - (long long)from * W;
+            if (t < a.k && t >= here) list[t] = 0;
+        }
+        const auto scan = [&](const auto &f) {
+            for (int c = from + t; c < to; c += T) {
+                const long long at = c * (long long)W, start = min(at, (long long)cols - W);
+                const Chunk<X, W> raw = load_chunk<X, W>(x + start);
+#pragma unroll
+                for (int i = 0; i < W; i++)
+                    if (start + i >= at) f(raw[i], c, (int)start + i);
+            }
+        };
+        team.top(a.k, most_at < 0 ? 0 : make_key(most, most_at), scan, [&](int rank, u64 key) {
+            if (p.parts == 1) put_top<PROBS>(a, r, row, rank, key);
+            else list[rank] = key;
+        });
+    }
+}
+
+// joins the parts of each row
+template <typename X, bool PROBS>
+__global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_args a, const Part p)
+{
+    __shared__ Team<kThreads>::Shared shared;
+    Team<kThreads> team(shared);
+    const int t = team.t;
+    for (size_t r = blockIdx.x; r < (size_t)a.rows; r += gridDim.x) {
+        const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        Stats s = {kLowest, 0.0f, 0.0f};
+        float least = 0.0f;
+        if (t < p.parts) {                          // (parts <= kThreads)
+            const float4 v = p.stats[r * p.parts + t];
+            s = {v.x, v.y, v.z};
+            least = v.w;
+        }
+        s = team.template join<PROBS>(s, least);
+        const Row row(s, least < 0.0f);
+        if (a.entropy && t == 0) a.entropy[r] = row.entropy();
+        if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
+        if (!wants_top(a)) continue;
+        if (row.bad) {
+            if (t < a.k) put_bad(a, r, t);
+            continue;
+        }
+        // the parts' lists: each thread takes every kThreads-th of their keys, a key being a chunk of its own (its column)
+        const u64 *keys = p.keys + r * p.parts * a.k;
+        const int n = p.parts * a.k;
+        u64 first = 0;
+        for (int i = t; i < n; i += kThreads) first = max(first, keys[i]);
+        const auto scan = [&](const auto &f) {
+            for (int i = t; i < n; i += kThreads)
+                if (const u64 key = keys[i]) f(key_value(key), key_column(key), key_column(key));
+        };
+        team.top(a.k, first, scan, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
+    }
+}
+
+// ---- which kernel, on what grid ----
+constexpr int kLongThreads = 512;
+constexpr int kMaxBlocks = 1 << 22;      // beyond it the workgroups take several rows each
+
+Part parts_of(int rows, int cols, int type)
+{
+    const int w = type == LCRC_T_F32 ? 4 : 8, n_chunks = (cols - 1) / w + 1;
+    // enough workgroups for every CU to have two, but no part below 4 chunks a thread (two rounds of loads are latency alone)
+    Part p = {1, n_chunks, nullptr, nullptr};
+    const long long most = std::min<long long>(kThreads, (n_chunks + 2 * kLongThreads - 1) / (2 * kLongThreads));
+    const long long want = rows >= 512 ? 1 : (512 + rows - 1) / rows;
+    const int parts = (int)std::max<long long>(1, std::min(most, want));
+    p.chunks = (n_chunks - 1) / parts + 1;
+    p.parts = (n_chunks - 1) / p.chunks + 1;
+    return p;
+}
+
+// rows of up to this many chunks of 16 bytes lie in a wave's registers
+constexpr int kWaveChunks = 8 * 64;
+
+size_t part_bytes(int rows, int cols, int k, int type)
+{
+    const int w = type == LCRC_T_F32 ? 4 : 8;
+    if ((cols - 1) / w + 1 <= kWaveChunks) return 0;
+    const Part p = parts_of(rows, cols, type);
+    return p.parts == 1 ? 0 : (size_t)rows * p.parts * (sizeof(float4) + (size_t)k * sizeof(u64));
+}
+
+template <typename X, bool PROBS, int W, int J>
+void launch_short(const lcrc_score_args &a, int k, hipStream_t stream)
+{
+    const int blocks = (int)std::min<long long>(((long long)a.rows + 15) / 16, kMaxBlocks);
+    if (k == 0) score_short_kernel<X, PROBS, W, J, 0><<<blocks, kThreads, 0, stream>>>(a);
+    else if (k == 1) score_short_kernel<X, PROBS, W, J, 1><<<blocks, kThreads, 0, stream>>>(a);
+    else if (k <= 3) score_short_kernel<X, PROBS, W, J, 3><<<blocks, kThreads, 0, stream>>>(a);
+    else if (k <= 5) score_short_kernel<X, PROBS, W, J, 5><<<blocks, kThreads, 0, stream>>>(a);
+    else score_short_kernel<X, PROBS, W, J, 8><<<blocks, kThreads, 0, stream>>>(a);
+}
+
+template <typename X, bool PROBS>
+hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
+{
+    constexpr int W = 16 / sizeof(X);
+    const int k = a.top_index || a.top_logp ? a.k : 0, chunks = (a.cols - 1) / W + 1;
+    if (a.cols < W) launch_short<X, PROBS, 1, 1>(a, k, stream);          // (k <= cols < 8)
+    else if (k <= 8 && chunks <= 16) launch_short<X, PROBS, W, 1>(a, k, stream);
+    else if (k <= 8 && chunks <= 32) launch_short<X, PROBS, W, 2>(a, k, stream);
+    else if (k <= 8 && chunks <= 48) launch_short<X, PROBS, W, 3>(a, k, stream);
+    else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 4>(a, k, stream);
+    else if (chunks <= kWaveChunks) {
+        const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, kMaxBlocks);
+        if (chunks <= 64) score_wave_kernel<X, PROBS, 1><<<blocks, kThreads, 0, stream>>>(a);
+        else if (chunks <= 128) score_wave_kernel<X, PROBS, 2><<<blocks, kThreads, 0, stream>>>(a);
+        else if (chunks <= 256) score_wave_kernel<X, PROBS, 4><<<blocks, kThreads, 0, stream>>>(a);
+        else score_wave_kernel<X, PROBS, 8><<<blocks, kThreads, 0, stream>>>(a);
+    } else {
+        Part p = parts_of(a.rows, a.cols, a.type);
+        const size_t jobs = (size_t)a.rows * p.parts;
+        p.stats = static_cast<float4 *>(a.workspace);
+        p.keys = reinterpret_cast<u64 *>(p.stats + (p.parts > 1 ? jobs : 0));
+        score_long_kernel<X, PROBS, kLongThreads><<<(int)std::min<size_t>(jobs, kMaxBlocks), kLongThreads, 0, stream>>>(a, p);
+        if (p.parts > 1) {
+            if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            score_join_kernel<X, PROBS><<<std::min(a.rows, kMaxBlocks), kThreads, 0, stream>>>(a, p);
+        }
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t score_workspace_bytes(int, int, int) { return 0; }
+size_t score_workspace_bytes(int rows, int cols, int k)
+{
+    // (of either width of type: the size function does not take the type)
+    return std::max(part_bytes(rows, cols, k, LCRC_T_F32), part_bytes(rows, cols, k, LCRC_T_BF16));
+}
 
 hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream)
 {
     const auto go = [&](auto x) {
-        if (a.form == LCRC_SCORE_PROBS) score_kernel<decltype(x), true><<<a.rows, kThreads, 0, stream>>>(a);
-        else score_kernel<decltype(x), false><<<a.rows, kThreads, 0, stream>>>(a);
+        typedef decltype(x) X;
+        return a.form == LCRC_SCORE_PROBS ? launch<X, true>(a, stream) : launch<X, false>(a, stream);
     };
-    if (a.type == LCRC_T_F32) go(float());
-    else if (a.type == LCRC_T_F16) go(_Float16());
-    else go(__bf16());
-    return hipGetLastError();
+    if (a.type == LCRC_T_F32) return go(float());
+    if (a.type == LCRC_T_F16) return go(_Float16());
+    return go(__bf16());
 }
 
 }  // namespace phnrec
