@@ -10,6 +10,7 @@
 // carries it; inf - inf is NaN), a negative posterior shows in the rows' minimum.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_dev.h"
 
@@ -97,12 +98,12 @@ __device__ __forceinline__ void add_value(float v, float m, float &S, float &T)
 template <bool PROBS>
 __device__ __forceinline__ float finish(float T) { return PROBS ? T * kLn2 : T; }
 
+template <bool PROBS>
 struct Row {
     float m, S, T, ln_s;
     bool bad, none;
     __device__ __forceinline__ Row(const Stats &s, bool negative)
-        : m(s.m), S(s.S), T(s.T), ln_s(logf(s.S)), bad(negative || !(s.S < INFINITY)), none(!(s.S > 0.0f)) {}
-    template <bool PROBS>
+        : m(s.m), S(s.S), T(s.T), ln_s(PROBS ? logf(s.S) : __builtin_amdgcn_logf(s.S) * kLn2), bad(negative || !(s.S < INFINITY)), none(!(s.S > 0.0f)) {}
     __device__ __forceinline__ float ln_p(float v) const
     {
         if (bad) return NAN;
@@ -113,10 +114,10 @@ struct Row {
 };
 
 template <typename X, bool PROBS>
-__device__ __forceinline__ float label_score(const lcrc_score_args &a, const X *x, const Row &row, size_t at)
+__device__ __forceinline__ float label_score(const lcrc_score_args &a, const X *x, const Row<PROBS> &row, size_t at)
 {
     const int c = a.labels[at];
-    return c < 0 ? 0.0f : c >= a.cols ? NAN : row.template ln_p<PROBS>(to_f32(x[c]));
+    return c < 0 ? 0.0f : c >= a.cols ? NAN : row.ln_p(to_f32(x[c]));
 }
 __device__ __forceinline__ bool wants_top(const lcrc_score_args &a) { return a.k > 0 && (a.top_index || a.top_logp); }
 
@@ -151,6 +152,9 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
         Chunk<X, W> raw[J];
 #pragma unroll
         for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((16 * j + lane) * W, cols - W));
+        // a lane's first label and its value: on their way while the row is worked on
+        const int label = a.logp && lane < a.n_labels ? a.labels[r * a.n_labels + lane] : -1;
+        const float labelled = to_f32(x[label < 0 || label >= cols ? 0 : label]);
         // (all chunks but the last J are whole)
         const int last = (16 * (J - 1) + lane) * W, start = min(last, cols - W);
         const auto live = [&](int j, int i) { return j < J - 1 || start + i >= last; };
@@ -175,10 +179,12 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
         s.S = reduce16(s.S, Add());
         s.T = finish<PROBS>(reduce16(s.T, Add()));
         if constexpr (PROBS) least = reduce16(least, Min());
-        const Row row(s, least < 0.0f);
+        const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
-        if (a.logp)
-            for (int j = lane; j < a.n_labels; j += 16) a.logp[r * a.n_labels + j] = label_score<X, PROBS>(a, x, row, r * a.n_labels + j);
+        if (a.logp && lane < a.n_labels)
+            a.logp[r * a.n_labels + lane] = label < 0 ? 0.0f : label >= cols ? NAN : row.ln_p(labelled);
+        if (a.logp && a.n_labels > 16)
+            for (int j = lane + 16; j < a.n_labels; j += 16) a.logp[r * a.n_labels + j] = label_score<X, PROBS>(a, x, row, r * a.n_labels + j);
         if constexpr (K > 0) {
             double best[K];
 #pragma unroll
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
             }
             if (lane < a.k) {
                 if (a.top_index) a.top_index[r * a.k + lane] = row.bad ? -1 : column_of(mine);
-                if (a.top_logp) a.top_logp[r * a.k + lane] = row.template ln_p<PROBS>(value_of(mine));
+                if (a.top_logp) a.top_logp[r * a.k + lane] = row.ln_p(value_of(mine));
             }
         }
     }
@@ -228,25 +234,44 @@ __device__ __forceinline__ float key_value(u64 k)
     return __uint_as_float(o ^ (~(unsigned)((int)o >> 31) | 0x80000000u));
 }
 
-// The k-th largest (1 <= k <= 64) of the 64 lanes' numbers, bit by bit from the top: a candidate stands if k lanes reach it.
-// One compare a bit on the vector side, the count on the scalar side.
-__device__ __forceinline__ unsigned kth_largest(unsigned v, int k, bool alive)
+// A bar that at least k (1 <= k <= 64) of the wave's 64 G keys reach, and no more than k where their upper halves differ:
+// bit by bit from the top, a candidate stands if k keys reach it, and the search ends when exactly k do.  One compare a bit and
+// key on the vector side, the count on the scalar side.  Equal upper halves (equal values) are told apart by the lower ones.
+template <int G>
+__device__ __forceinline__ int count_from(const unsigned (&v)[G], unsigned t)
+{
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < G; q++) n += __popcll(__ballot(v[q] >= t));
+    return n;
+}
+template <int G>
+__device__ __forceinline__ unsigned bar_of(const unsigned (&v)[G], int k, int *reached)
 {
     unsigned res = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    int n = 64 * G;
+    for (int bit = 31; bit >= 0 && n != k; bit--) {
         const unsigned t = res | (1u << bit);
-        if (__popcll(__ballot(alive && v >= t)) >= k) res = t;
+        const int c = count_from(v, t);
+        if (c >= k) res = t, n = c;
     }
+    *reached = n;
     return res;
 }
-__device__ __forceinline__ u64 kth_largest(u64 key, int k)
+template <int G>
+__device__ __forceinline__ u64 bar_of(const u64 (&key)[G], int k)
 {
-    const unsigned hi = (unsigned)(key >> 32), lo = (unsigned)key;
-    const unsigned h = kth_largest(hi, k, true);
-    const int more = __popcll(__ballot(hi > h));
-    unsigned l = 0;
-    if (__popcll(__ballot(hi >= h)) > k) l = kth_largest(lo, k - more, hi == h);
-    return ((u64)h << 32) | l;
+    unsigned hi[G], lo[G];
+#pragma unroll
+    for (int q = 0; q < G; q++) hi[q] = (unsigned)(key[q] >> 32);
+    int n;
+    const unsigned h = bar_of(hi, k, &n);
+    if (n == k || h == 0) return (u64)h << 32;
+    // more than k: they stand at exactly h or above (all bits are decided); the lower half decides among those at h
+    const int more = h == 0xffffffffu ? 0 : count_from(hi, h + 1);
+#pragma unroll
+    for (int q = 0; q < G; q++) lo[q] = hi[q] == h ? (unsigned)key[q] : 0;
+    return ((u64)h << 32) | bar_of(lo, k - more, &n);
 }
 
 constexpr int kCandidates = 512;       // candidates a team holds (more: the slow way)
@@ -325,32 +350,38 @@ struct Team {
         }
         return v;
     }
-    // The k best of the team's keys, best first: out(rank, key), by the thread that finds it.
-    //   first          this thread's best (value, chunk) as a key, 0 if it has none
-    //   scan(f)        f(value, chunk, column) for all that this thread holds
-    // The threads are put into 64 groups.  The k-th best of the groups' bests is reached by at least k values, so the k best
-    // are among the values that reach it, and those lie with the k groups that do: only their threads look at their values
-    // again.  The few that remain are ranked by counting.  Rows made so that more remain than fit are done one rank after
-    // another.
-    template <typename Scan, typename Out>
-    __device__ __forceinline__ void top(int k, u64 first, const Scan &scan, const Out &out)
+    // The k best of the team's values, best first: out(rank, key), by the thread that finds it.
+    //   first          the bests (value, chunk) of this thread's shares, as keys, 0 where it has none
+    //   scan(bar, f)   f(value, chunk, column) for what this thread holds, at least for the values whose keys reach the bar
+    // The threads' shares are put into 64 G groups.  The k-th best of the groups' bests is reached by at least k values, so
+    // the k best are among the values that reach it, and only threads with such a group look at their values again.  With
+    // 256 groups some 74 of random values remain for k = 64, 17 for k = 16 (from 64 groups 300 and 18).  They are ranked by
+    // counting.  Rows made so that more remain than fit are done one rank after another.
+    template <int N, typename Scan, typename Out>
+    __device__ __forceinline__ void top(int k, const u64 (&first)[N], const Scan &scan, const Out &out)
     {
-        u64 group = first;
+        constexpr int G = T > 64 ? 4 : N;
+        u64 group[G];
+        if (t == 0) sh.count = 0;
         if constexpr (T > 64) {
-            sh.best[t] = first;
-            if (t == 0) sh.count = 0;
+            sh.best[t] = first[0];
             sync();
-            for (int w = 0; w < kWaves; w++) {
-                const u64 o = sh.best[64 * w + (t & 63)];
-                group = o > group ? o : group;
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                group[q] = 0;
+                for (int w = q; w < kWaves; w += G) group[q] = max(group[q], sh.best[64 * w + (t & 63)]);
             }
         } else {
-            if (t == 0) sh.count = 0;
+#pragma unroll
+            for (int q = 0; q < G; q++) group[q] = first[q];
             sync();
         }
-        const u64 bar = kth_largest(group, k);
-        if (first >= bar && first != 0)
-            scan([&](float v, int chunk, int c) {
+        const u64 bar = bar_of(group, k);
+        bool look = false;
+#pragma unroll
+        for (int q = 0; q < N; q++) look = look || (first[q] >= bar && first[q] != 0);
+        if (look)
+            scan(bar, [&](float v, int chunk, int c) {
                 if (make_key(v, chunk) >= bar) {
                     const int at = atomicAdd(&sh.count, 1);      // (any order: they are ranked by their keys)
                     if (at < kCandidates) sh.cand[at] = make_key(v, c);
@@ -362,6 +393,7 @@ struct Team {
             for (int i = t; i < n; i += T) {
                 const u64 key = sh.cand[i];
                 int rank = 0;
+#pragma unroll 8
                 for (int q = 0; q < n; q++) rank += sh.cand[q] > key ? 1 : 0;
                 if (rank < k) out(rank, key);
             }
@@ -369,7 +401,7 @@ struct Team {
             u64 last = ~0ull;
             for (int q = 0; q < k; q++) {
                 u64 best = 0;
-                scan([&](float v, int, int c) {
+                scan(0, [&](float v, int, int c) {
                     const u64 key = make_key(v, c);
                     if (key < last && key > best) best = key;
                 });
@@ -387,10 +419,10 @@ __device__ __forceinline__ void put_bad(const lcrc_score_args &a, size_t r, int 
     if (a.top_logp) a.top_logp[r * a.k + rank] = NAN;
 }
 template <bool PROBS>
-__device__ __forceinline__ void put_top(const lcrc_score_args &a, size_t r, const Row &row, int rank, u64 key)
+__device__ __forceinline__ void put_top(const lcrc_score_args &a, size_t r, const Row<PROBS> &row, int rank, u64 key)
 {
     if (a.top_index) a.top_index[r * a.k + rank] = key_column(key);
-    if (a.top_logp) a.top_logp[r * a.k + rank] = row.template ln_p<PROBS>(key_value(key));
+    if (a.top_logp) a.top_logp[r * a.k + rank] = row.ln_p(key_value(key));
 }
 
 // ---- middle rows: a wave to a row, the row in its registers: J chunks of 16 bytes to a lane ----
@@ -432,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
         s.S = reduce64(s.S, Add());
         s.T = finish<PROBS>(reduce64(s.T, Add()));
         if constexpr (PROBS) least = reduce64(least, Min());
-        const Row row(s, least < 0.0f);
+        const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
         if (a.logp && lane < a.n_labels) a.logp[r * a.n_labels + lane] = label_score<X, PROBS>(a, x, row, r * a.n_labels + lane);
         if (!wants_top(a)) continue;
@@ -440,12 +472,13 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
             if (lane < a.k) put_bad(a, r, lane);
             continue;
         }
-        u64 first = 0;
+        constexpr int N = J > 1 ? 2 : 1;
+        u64 first[N] = {};
         each([&](float v, int chunk, int) {
-            const u64 key = make_key(v, chunk);
-            first = key > first ? key : first;
+            u64 &f = first[(chunk >> 6) % N];
+            f = max(f, make_key(v, chunk));
         });
-        team.top(a.k, first, each, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
+        team.top(a.k, first, [&](u64, const auto &f) { each(f); }, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
     }
 }
 
@@ -471,28 +504,32 @@ __global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, 
         const int from = (int)(job - r * p.parts) * p.chunks, to = min(from + p.chunks, n_chunks);
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
         Stats s = {kLowest, 0.0f, 0.0f};
-        float least = 0.0f, most = -INFINITY;
+        float least = 0.0f, most = -INFINITY, second = -INFINITY;       // the best chunk, and the best value of the others
         int most_at = -1;
-        for (int c0 = from + t; c0 < to; c0 += U * T) {
+        // U chunks, T apart; CHECKED: some of them may lie behind the part's end or be the row's last one
+        const auto take = [&](int c0, auto checked) {
+            constexpr bool CHECKED = decltype(checked)::value;
             Chunk<X, W> raw[U];
-            bool whole[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) raw[u] = load_chunk<X, W>(x + min((c0 + u * T) * (long long)W, (long long)cols - W));
+            for (int u = 0; u < U; u++) {
+                const long long at = (c0 + u * T) * (long long)W;
+                raw[u] = load_chunk<X, W>(x + (CHECKED ? min(at, (long long)cols - W) : at));
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int c = c0 + u * T;
-                whole[u] = c < to;
-                if (!whole[u]) continue;
+                if (CHECKED && c >= to) break;
+                // (values that the row's last chunk shares with the one before it are that one's)
+                const int twice = CHECKED ? (int)max(0ll, (c + 1) * (long long)W - cols) : 0;
                 float v = raw[u][W - 1];
-                const int twice = (int)max(0ll, (c + 1) * (long long)W - cols);       // of the row's last chunk
 #pragma unroll
                 for (int i = 0; i < W - 1; i++)
                     if (i >= twice) v = fmaxf(v, raw[u][i]);
-                if (v > most || most_at < 0) {
-                    most = v;
-                    most_at = c;
-                }
+                const bool better = v > most || most_at < 0;
+                second = fmaxf(second, better ? most : v);
+                most = better ? v : most;
+                most_at = better ? c : most_at;
                 top = fmaxf(top, v);
             }
             if constexpr (!PROBS)
@@ -504,27 +541,24 @@ __global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, 
                 }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                if (!whole[u]) continue;
-                const long long at = (c0 + u * T) * (long long)W;
-                if (at + W <= cols) {
+                const int c = c0 + u * T;
+                if (CHECKED && c >= to) break;
+                const int twice = CHECKED ? (int)max(0ll, (c + 1) * (long long)W - cols) : 0;
 #pragma unroll
-                    for (int i = 0; i < W; i++) {
-                        if constexpr (PROBS) least = fminf(least, raw[u][i]);
-                        add_value<PROBS>(raw[u][i], s.m, s.S, s.T);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < W; i++)
-                        if (cols - W + i >= at) {
-                            if constexpr (PROBS) least = fminf(least, raw[u][i]);
-                            add_value<PROBS>(raw[u][i], s.m, s.S, s.T);
-                        }
+                for (int i = 0; i < W; i++) {
+                    const float v = i >= twice ? raw[u][i] : PROBS ? 0.0f : -INFINITY;
+                    if constexpr (PROBS) least = fminf(least, v);
+                    add_value<PROBS>(v, s.m, s.S, s.T);
                 }
             }
-        }
+        };
+        const int whole = min(to, cols / W);        // chunks before it need no checks
+        int c0 = from + t;
+        for (; c0 - t + U * T <= whole; c0 += U * T) take(c0, std::false_type());
+        for (; c0 < to; c0 += U * T) take(c0, std::true_type());
         s.T = finish<PROBS>(s.T);
         s = team.template join<PROBS>(s, least);
-        const Row row(s, least < 0.0f);
+        const Row<PROBS> row(s, least < 0.0f);
         if (p.parts == 1) {
             if (a.entropy && t == 0) a.entropy[r] = row.entropy();
             if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
@@ -540,16 +574,30 @@ __global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, 
             const long long here = min((long long)to * W, (long long)cols) - (long long)from * W;
             if (t < a.k && t >= here) list[t] = 0;
         }
-        const auto scan = [&](const auto &f) {
-            for (int c = from + t; c < to; c += T) {
-                const long long at = c * (long long)W, start = min(at, (long long)cols - W);
-                const Chunk<X, W> raw = load_chunk<X, W>(x + start);
+        const auto look_at = [&](const Chunk<X, W> &raw, int c, const auto &f) {
+            const long long at = c * (long long)W, start = min(at, (long long)cols - W);
 #pragma unroll
-                for (int i = 0; i < W; i++)
-                    if (start + i >= at) f(raw[i], c, (int)start + i);
+            for (int i = 0; i < W; i++)
+                if (start + i >= at) f(raw[i], c, (int)start + i);
+        };
+        const auto chunk = [&](int c) { return load_chunk<X, W>(x + min(c * (long long)W, (long long)cols - W)); };
+        // bar: what f is looking for; mostly a thread has it in its best chunk alone
+        const auto scan = [&](u64 bar, const auto &f) {
+            if (ordered(second) < (unsigned)(bar >> 32)) {
+                if (most_at >= 0) look_at(chunk(most_at), most_at, f);
+                return;
+            }
+            for (int c = from + t; c < to; c += U * T) {
+                Chunk<X, W> raw[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) raw[u] = chunk(min(c + u * T, to - 1));
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (c + u * T < to) look_at(raw[u], c + u * T, f);
             }
         };
-        team.top(a.k, most_at < 0 ? 0 : make_key(most, most_at), scan, [&](int rank, u64 key) {
+        const u64 first[1] = {most_at < 0 ? 0 : make_key(most, most_at)};
+        team.top(a.k, first, scan, [&](int rank, u64 key) {
             if (p.parts == 1) put_top<PROBS>(a, r, row, rank, key);
             else list[rank] = key;
         });
@@ -573,7 +621,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
             least = v.w;
         }
         s = team.template join<PROBS>(s, least);
-        const Row row(s, least < 0.0f);
+        const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && t == 0) a.entropy[r] = row.entropy();
         if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
         if (!wants_top(a)) continue;
@@ -581,14 +629,15 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
             if (t < a.k) put_bad(a, r, t);
             continue;
         }
-        // the parts' lists: each thread takes every kThreads-th of their keys, a key being a chunk of its own (its column)
+        // the parts' lists, rank by rank: the best ones lie with different threads; a key is a chunk of its own (its column)
         const u64 *keys = p.keys + r * p.parts * a.k;
         const int n = p.parts * a.k;
-        u64 first = 0;
-        for (int i = t; i < n; i += kThreads) first = max(first, keys[i]);
-        const auto scan = [&](const auto &f) {
+        const auto key_at = [&](int i) { return keys[i % p.parts * a.k + i / p.parts]; };
+        u64 first[1] = {};
+        for (int i = t; i < n; i += kThreads) first[0] = max(first[0], key_at(i));
+        const auto scan = [&](u64, const auto &f) {
             for (int i = t; i < n; i += kThreads)
-                if (const u64 key = keys[i]) f(key_value(key), key_column(key), key_column(key));
+                if (const u64 key = key_at(i)) f(key_value(key), key_column(key), key_column(key));
         };
         team.top(a.k, first, scan, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
     }
