@@ -1,6 +1,8 @@
 // fp8_kernels.hip -- matrices held in e4m3 with a power-of-two scale for each block of 128 columns (ops_dev.h: the form), and
 // their products on the block-scaled matrix instructions (include/lcrc_pipeline.h: lcrc_fp8_pack / _unpack / _linear).
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_dev.h"
 
@@ -73,6 +75,25 @@ __device__ __forceinline__ i8 load_tile(const unsigned char *tile, int lane)
     return i8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+// a lane's 32 values of block kb of a row: four at a time where the block is whole
+template <typename X>
+__device__ __forceinline__ void load_block(const X *row, bool live, long long kb, int cols, int g, float (&v)[32])
+{
+    if ((kb + 1) * 128 <= cols) {
+        struct Four { X v[4]; } f[8];
+#pragma unroll
+        for (int w = 0; w < 8; w++) __builtin_memcpy(&f[w], row + kb * 128 + column_of(g, 4 * w), sizeof(Four));
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = live ? to_f32(f[j >> 2].v[j & 3]) : 0.0f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const long long k = kb * 128 + column_of(g, j);
+            v[j] = live && k < cols ? to_f32(row[k]) : 0.0f;
+        }
+    }
+}
+
 // One wave per tile of 16 rows x 128 columns.
 template <typename X>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
@@ -102,11 +123,7 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
     } else {
         const X *src = static_cast<const X *>(p.src) + (live ? row : 0) * p.ld;
         float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const long long k = kb * 128 + column_of(g, j);
-            v[j] = live && k < p.cols ? to_f32(src[k]) : 0.0f;
-        }
+        load_block(src, live, kb, p.cols, g, v);
         q = quantise(v, &e);
     }
     store_tile(p.dst + tile * kQTileBytes, lane, q);
@@ -140,18 +157,30 @@ __global__ __launch_bounds__(256) void fp8_unpack_kernel(const Fp8UnpackParams p
     }
 }
 
-template <int ACT>
-__device__ __forceinline__ float activate(float v)
+// LCRC_ACT_SIGMOID on the hardware's 2^x and reciprocal (1 ulp each)
+__device__ __forceinline__ float sigmoid(float v)
 {
-    if constexpr (ACT == LCRC_ACT_SIGMOID) return 1.0f / (1.0f + expf(-v));
-    if constexpr (ACT == LCRC_ACT_FSIGMOID) {
-        // FEXP (fexp.h:14-21): the exponent's bits of a double from one truncated product; out of range as x86 converts it
-        const float y = -v;
-        int i = __double2int_rz(1048576.0 / 0.69314718055994530942 * (double)y);
-        if (!(y < 0x1.62e43p+10f)) i = (int)0x80000000u;
-        return 1.0f / (1.0f + (float)__hiloint2double((int)((unsigned)i + 1072632447u), 0));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+}
+// LCRC_ACT_FSIGMOID.  FEXP (fexp.h:14-21): the exponent's bits of a double from one truncated product; out of range as x86
+// converts it
+__device__ __forceinline__ float fsigmoid(float v)
+{
+    const float y = -v;
+    int i = __double2int_rz(1048576.0 / 0.69314718055994530942 * (double)y);
+    if (!(y < 0x1.62e43p+10f)) i = (int)0x80000000u;
+    return 1.0f / (1.0f + (float)__hiloint2double((int)((unsigned)i + 1072632447u), 0));
+}
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act)
+{
+    if (act == LCRC_ACT_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = sigmoid(v[i]);
+    } else if (act == LCRC_ACT_FSIGMOID) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = fsigmoid(v[i]);
     }
-    return v;
 }
 
 // ---- the sums ----
@@ -188,79 +217,173 @@ __device__ __forceinline__ f4 block_product(const i8 &a, const i8 &b, f4 acc, in
     return acc;
 }
 
-// D = W X^T per tile of 16 x 16: lane (c, g) holds features 4 g + r (register r) of x row c.
-// One wave per 16 rows x 128 outputs, operands straight from memory.
-template <int ACT, typename Y>
-__global__ __launch_bounds__(256) void fp8_product_kernel(const Fp8ProductParams p)
+// D = W X^T per tile of 16 x 16: lane (c, g) holds outputs 4 g + r (register r) of x row c.
+
+// four outputs o .. o + 3 of a row, as they lie in a lane; o is a multiple of 4
+template <typename Y>
+__device__ __forceinline__ void store_four(Y *row, long long o, int n_out, const float *v)
 {
-    const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= sx.rt * sy.kb) return;
-    const long long t = id / sy.kb, ob = id % sy.kb;                   // row tile, block of 128 outputs
-    const unsigned char *x = p.x + t * sx.kb * kQTileBytes;
-    const int *xs = reinterpret_cast<const int *>(p.x + sx.scales_at()) + t * sx.kb4 * 16 + c;
-    const unsigned char *w[8];
-    const int *ws[8];
-#pragma unroll
-    for (int n = 0; n < 8; n++) {
-        const long long wt = min(8 * ob + n, sw.rt - 1);
-        w[n] = p.w + wt * sw.kb * kQTileBytes;
-        ws[n] = reinterpret_cast<const int *>(p.w + sw.scales_at()) + wt * sw.kb4 * 16 + c;
-    }
-    f4 acc[8];
-#pragma unroll
-    for (int n = 0; n < 8; n++) acc[n] = f4{0.f, 0.f, 0.f, 0.f};
-    for (long long kb = 0; kb < sx.kb; kb++) {
-        const i8 b = load_tile(x + kb * kQTileBytes, lane);
-        const int shift = 8 * (int)(kb & 3);
-        const int bs = xs[(kb >> 2) * 16] >> shift;
-#pragma unroll
-        for (int n = 0; n < 8; n++) {
-            const i8 a = load_tile(w[n] + kb * kQTileBytes, lane);
-            const int as = ws[n][(kb >> 2) * 16] >> shift;
-            acc[n] = block_product<sizeof(Y) == 4>(a, b, acc[n], as, bs);
-        }
-    }
-    const long long row = 16 * t + c;
-    float v[32];
-#pragma unroll
-    for (int n = 0; n < 8; n++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const long long o = 128 * ob + 16 * n + 4 * g + r;
-            const bool live = row < p.rows && o < p.n_out;
-            v[4 * n + r] = live ? activate<ACT>(acc[n][r] + (p.bias ? p.bias[o] : 0.0f)) : 0.0f;
-        }
-    if constexpr (sizeof(Y) == 1) {
-        unsigned char *y = static_cast<unsigned char *>(p.y);
-        int e;
-        const i8 q = quantise(v, &e);
-        store_tile(y + (t * sy.kb + ob) * kQTileBytes, lane, q);
-        unsigned char *scales = y + sy.scales_at() + ((t * sy.kb4 + ob / 4) * 16 + c) * 4;
-        if (g == 0) scales[ob & 3] = (unsigned char)(e + 127);
-        if (ob == sy.kb - 1 && g > (ob & 3)) scales[g] = 127;
+    if (o + 4 <= n_out) {
+        struct Four { Y v[4]; } f = {{(Y)v[0], (Y)v[1], (Y)v[2], (Y)v[3]}};
+        __builtin_memcpy(row + o, &f, sizeof(f));
     } else {
-        Y *y = static_cast<Y *>(p.y) + row * p.ldy;
 #pragma unroll
-        for (int n = 0; n < 8; n++)
+        for (int r = 0; r < 4; r++)
+            if (o + r < n_out) row[o + r] = (Y)v[r];
+    }
+}
+__device__ __forceinline__ void store_rows(const Fp8ProductParams &p, long long row, long long o, const float *v)
+{
+    if (row >= p.rows) return;
+    if (p.y_type == LCRC_T_F32) store_four(static_cast<float *>(p.y) + row * p.ldy, o, p.n_out, v);
+    else if (p.y_type == LCRC_T_F16) store_four(static_cast<_Float16 *>(p.y) + row * p.ldy, o, p.n_out, v);
+    else store_four(static_cast<__bf16 *>(p.y) + row * p.ldy, o, p.n_out, v);
+}
+__device__ __forceinline__ void add_bias(const Fp8ProductParams &p, long long o, float *v)
+{
+    if (!p.bias) return;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const long long o = 128 * ob + 16 * n + 4 * g + r;
-                if (row < p.rows && o < p.n_out) y[o] = (Y)v[4 * n + r];
-            }
+    for (int r = 0; r < 4; r++)
+        if (o + r < p.n_out) v[r] += p.bias[o + r];
+}
+// a lane's 32 outputs of row 16 t + c, block ob of 128, as the tile (t, ob) of the 8-bit form; what fills it up is 0
+__device__ __forceinline__ void store_held(const Fp8ProductParams &p, const Q8Shape &sy, long long t, long long ob, int lane, float (&v)[32])
+{
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+        if (16 * t + c >= p.rows || 128 * ob + column_of(g, j) >= p.n_out) v[j] = 0.0f;
+    unsigned char *y = static_cast<unsigned char *>(p.y);
+    int e;
+    const i8 q = quantise(v, &e);
+    store_tile(y + (t * sy.kb + ob) * kQTileBytes, lane, q);
+    unsigned char *scales = y + sy.scales_at() + ((t * sy.kb4 + ob / 4) * 16 + c) * 4;
+    if (g == 0) scales[ob & 3] = (unsigned char)(e + 127);
+    if (ob == sy.kb - 1 && g > (ob & 3)) scales[g] = 127;
+}
+
+typedef const unsigned char __attribute__((address_space(1))) *global_bytes;
+typedef unsigned char __attribute__((address_space(3))) *lds_bytes;
+
+// block J of a group of four, scale bytes J of the groups' dwords
+template <bool EXACT, int J>
+__device__ __forceinline__ f4 scaled_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
+{
+    if constexpr (EXACT) return block_product<true>(a, b, acc, as >> (8 * J), bs >> (8 * J));
+    else return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, J, as, J, bs);
+}
+
+// A workgroup of WW x WX waves makes 16 FW WW outputs of 16 FX WX rows, each wave FW x FX tiles in its registers.
+template <bool EXACT, int FW, int FX, int WW, int WX>
+__global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
+{
+    constexpr int kWaves = WW * WX, TW = FW * WW, TX = FX * WX, PW = 2 * TW / kWaves, PX = 2 * TX / kWaves, kPiece = kQTileBytes / 2;
+    static_assert(FW == 8 && PW * kWaves == 2 * TW && PX * kWaves == 2 * TX, "whole blocks of outputs; the copies are shared out evenly");
+    __shared__ __attribute__((aligned(16))) unsigned char stage[(TW + TX) * kQTileBytes];
+    const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
+    const int lane = threadIdx.x & 63, c = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ww = wave % WW, wx = wave / WW;
+    // Workgroup i runs on XCD i mod 8, each with an L2 of its own: an XCD takes a run of neighbouring tiles, eight rows of
+    // tiles by columns, so that what runs together shares its operands.
+    const long long all = (long long)across * down, per = (all + 7) / 8;
+    const long long id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || id >= all) return;
+    const long long band = id / (8ll * across), in_band = id - band * 8 * across, high = min(8ll, down - band * 8);
+    const long long tx = band * 8 + in_band % high, tw = in_band / high;
+
+    // the copies of a wave: pieces of 1 KB, half a tile, from where they lie behind the workgroup's first tile (n_in <= 2^23:
+    // within 32 bits)
+    const unsigned char *const w0 = p.w + tw * TW * sw.kb * kQTileBytes, *const x0 = p.x + tx * TX * sx.kb * kQTileBytes;
+    const int w_left = (int)min(sw.rt - tw * TW, (long long)TW) - 1, x_left = (int)min(sx.rt - tx * TX, (long long)TX) - 1;
+    const unsigned tile_stride = (unsigned)sx.kb * kQTileBytes, scale_stride = (unsigned)sx.kb4 * 64;
+    unsigned wp[PW], xp[PX];
+#pragma unroll
+    for (int q = 0; q < PW; q++) wp[q] = min((wave * PW + q) >> 1, w_left) * tile_stride + (q & 1) * kPiece + lane * 16;
+#pragma unroll
+    for (int q = 0; q < PX; q++) xp[q] = min((wave * PX + q) >> 1, x_left) * tile_stride + (q & 1) * kPiece + lane * 16;
+    const auto fetch = [&](long long kb) {                  // block kb of the operands into the stage, past the registers
+#pragma unroll
+        for (int q = 0; q < PW; q++)
+            __builtin_amdgcn_global_load_lds((global_bytes)(w0 + kb * kQTileBytes + wp[q]), (lds_bytes)(stage + (wave * PW + q) * kPiece), 16, 0, 0);
+#pragma unroll
+        for (int q = 0; q < PX; q++)
+            __builtin_amdgcn_global_load_lds((global_bytes)(x0 + kb * kQTileBytes + xp[q]), (lds_bytes)(stage + (2 * TW + wave * PX + q) * kPiece), 16, 0, 0);
+    };
+    const unsigned char *const ws = p.w + sw.scales_at() + tw * TW * sw.kb4 * 64, *const xs = p.x + sx.scales_at() + tx * TX * sx.kb4 * 64;
+    int s[FW + FX];
+    const auto fetch_scales = [&](long long kb4) {          // of four blocks: a dword for each row
+#pragma unroll
+        for (int n = 0; n < FW; n++)
+            s[n] = *reinterpret_cast<const int *>(ws + kb4 * 64 + min(ww * FW + n, w_left) * scale_stride + c * 4);
+#pragma unroll
+        for (int n = 0; n < FX; n++)
+            s[FW + n] = *reinterpret_cast<const int *>(xs + kb4 * 64 + min(wx * FX + n, x_left) * scale_stride + c * 4);
+    };
+
+    f4 acc[FW][FX];
+#pragma unroll
+    for (int n = 0; n < FW; n++)
+#pragma unroll
+        for (int m = 0; m < FX; m++) acc[n][m] = f4{0.f, 0.f, 0.f, 0.f};
+    const auto step = [&](long long kb, auto j) {
+        constexpr int J = decltype(j)::value;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's copies have arrived (a barrier alone does not wait for them)
+        __syncthreads();                                    // ... and everyone's
+        i8 a[FW], b[FX];
+#pragma unroll
+        for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
+#pragma unroll
+        for (int n = 0; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                       // ... and read by all
+        if (kb + 1 < sx.kb) fetch(kb + 1);                  // on its way while the products run
+#pragma unroll
+        for (int n = 0; n < FW; n++)
+#pragma unroll
+            for (int m = 0; m < FX; m++) acc[n][m] = scaled_product<EXACT, J>(a[n], b[m], acc[n][m], s[n], s[FW + m]);
+    };
+    fetch(0);
+    fetch_scales(0);
+    for (long long kb = 0; kb < sx.kb; kb += 4) {
+        step(kb, std::integral_constant<int, 0>());
+        if (kb + 1 < sx.kb) step(kb + 1, std::integral_constant<int, 1>());
+        if (kb + 2 < sx.kb) step(kb + 2, std::integral_constant<int, 2>());
+        if (kb + 3 < sx.kb) step(kb + 3, std::integral_constant<int, 3>());
+        if (kb + 4 < sx.kb) fetch_scales(kb / 4 + 1);
+    }
+
+    const long long ob = tw * WW + ww;                      // the wave's block of 128 outputs
+#pragma unroll
+    for (int m = 0; m < FX; m++) {
+        const long long t = tx * TX + wx * FX + m;
+        float v[32];
+#pragma unroll
+        for (int n = 0; n < FW; n++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[4 * n + r] = acc[n][m][r];
+            add_bias(p, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
+        }
+        activate(v, p.act);
+        if (p.y_type == LCRC_T_E4M3) {
+            if (t < sy.rt && ob < sy.kb) store_held(p, sy, t, ob, lane, v);
+        } else {
+#pragma unroll
+            for (int n = 0; n < FW; n++) store_rows(p, 16 * t + c, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
+        }
     }
 }
 
-template <int ACT>
-void product_by_type(const Fp8ProductParams &p, unsigned blocks, hipStream_t stream)
+template <bool EXACT, int FW, int FX, int WW, int WX>
+void tile_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
-    switch (p.y_type) {
-    case LCRC_T_F32: fp8_product_kernel<ACT, float><<<blocks, 256, 0, stream>>>(p); break;
-    case LCRC_T_F16: fp8_product_kernel<ACT, _Float16><<<blocks, 256, 0, stream>>>(p); break;
-    case LCRC_T_BF16: fp8_product_kernel<ACT, __bf16><<<blocks, 256, 0, stream>>>(p); break;
-    default: fp8_product_kernel<ACT, unsigned char><<<blocks, 256, 0, stream>>>(p); break;
-    }
+    const long long across = ((long long)p.n_out + 16 * FW * WW - 1) / (16 * FW * WW), down = ((long long)p.rows + 16 * FX * WX - 1) / (16 * FX * WX);
+    const long long blocks = (across * down + 7) / 8 * 8;
+    fp8_tile_kernel<EXACT, FW, FX, WW, WX><<<(unsigned)blocks, 64 * WW * WX, 0, stream>>>(p, (int)across, (int)down);
+}
+// tiles of 16 FW WW outputs x 16 FX WX rows
+long long tiles(const Fp8ProductParams &p, int outputs, int rows)
+{
+    return (((long long)p.n_out + outputs - 1) / outputs) * (((long long)p.rows + rows - 1) / rows);
 }
 
 }  // namespace
@@ -292,13 +415,12 @@ hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream)
 
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
-    const Q8Shape sx(p.rows, p.n_in), sy(p.rows, p.n_out);
-    const unsigned blocks = (unsigned)((sx.rt * sy.kb + 3) / 4);
-    switch (p.act) {
-    case LCRC_ACT_NONE: product_by_type<LCRC_ACT_NONE>(p, blocks, stream); break;
-    case LCRC_ACT_SIGMOID: product_by_type<LCRC_ACT_SIGMOID>(p, blocks, stream); break;
-    default: product_by_type<LCRC_ACT_FSIGMOID>(p, blocks, stream); break;
-    }
+    if (p.y_type == LCRC_T_F32) {
+        if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4>(p, stream);
+        else tile_launch<true, 8, 1, 1, 4>(p, stream);
+    } else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
+    else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4>(p, stream);
+    else tile_launch<false, 8, 1, 1, 4>(p, stream);
     return hipGetLastError();
 }
 
