@@ -75,24 +75,48 @@ __device__ __forceinline__ i8 load_tile(const unsigned char *tile, int lane)
     return i8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// a lane's 32 values of block kb of a row: four at a time where the block is whole
+// A lane's 32 values of block kb of a row, four at a time.  In a block that the row's end cuts off, a group of four that would
+// pass the end is read so that it ends there and moved into place afterwards.
 template <typename X>
-__device__ __forceinline__ void load_block(const X *row, bool live, long long kb, int cols, int g, float (&v)[32])
-{
-    if ((kb + 1) * 128 <= cols) {
-        struct Four { X v[4]; } f[8];
+struct RawBlock {
+    struct Four { X v[4]; } f[8];
+    static __device__ __forceinline__ int moved(int w, int g, int left) { return max(16 * w + 4 * g + 4 - left, 0); }
+    __device__ __forceinline__ void load(const X *row, long long kb, int cols, int g)
+    {
+        const X *x = row + kb * 128;
+        const int left = (int)min((long long)cols - kb * 128, 128ll);
+        if (cols >= 4) {
 #pragma unroll
-        for (int w = 0; w < 8; w++) __builtin_memcpy(&f[w], row + kb * 128 + column_of(g, 4 * w), sizeof(Four));
+            for (int w = 0; w < 8; w++) __builtin_memcpy(&f[w], x + (16 * w + 4 * g - moved(w, g, left)), sizeof(Four));
+        } else {
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = live ? to_f32(f[j >> 2].v[j & 3]) : 0.0f;
-    } else {
+            for (int w = 0; w < 8; w++)
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const long long k = kb * 128 + column_of(g, j);
-            v[j] = live && k < cols ? to_f32(row[k]) : 0.0f;
+                for (int r = 0; r < 4; r++) f[w].v[r] = w == 0 ? x[min(r, cols - 1)] : X(0);
         }
     }
-}
+    // live: the row exists
+    __device__ __forceinline__ void values(float (&out)[32], bool live, long long kb, int cols, int g) const
+    {
+        const int left = (int)min((long long)cols - kb * 128, 128ll);
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = live ? to_f32(f[w].v[r]) : 0.0f;
+            if (left < 128) {
+                const int by = cols >= 4 ? moved(w, g, left) : 0;
+                if (by & 1) v[0] = v[1], v[1] = v[2], v[2] = v[3];
+                if (by & 2) v[0] = v[2], v[1] = v[3];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (16 * w + 4 * g + r >= left) v[r] = 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) out[4 * w + r] = v[r];
+        }
+    }
+};
 
 // One wave per tile of 16 rows x 128 columns.
 template <typename X>
@@ -123,7 +147,9 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
     } else {
         const X *src = static_cast<const X *>(p.src) + (live ? row : 0) * p.ld;
         float v[32];
-        load_block(src, live, kb, p.cols, g, v);
+        RawBlock<X> raw;
+        raw.load(src, kb, p.cols, g);
+        raw.values(v, live, kb, p.cols, g);
         q = quantise(v, &e);
     }
     store_tile(p.dst + tile * kQTileBytes, lane, q);
@@ -239,12 +265,16 @@ __device__ __forceinline__ void store_rows(const Fp8ProductParams &p, long long 
     else if (p.y_type == LCRC_T_F16) store_four(static_cast<_Float16 *>(p.y) + row * p.ldy, o, p.n_out, v);
     else store_four(static_cast<__bf16 *>(p.y) + row * p.ldy, o, p.n_out, v);
 }
-__device__ __forceinline__ void add_bias(const Fp8ProductParams &p, long long o, float *v)
+// the bias of outputs o .. o + 3 (0 without one; what lies behind the last output is not used)
+__device__ __forceinline__ f4 bias_of(const Fp8ProductParams &p, long long o)
 {
-    if (!p.bias) return;
+    f4 b = {0.f, 0.f, 0.f, 0.f};
+    if (!p.bias) return b;
+    if (o + 4 <= p.n_out) __builtin_memcpy(&b, p.bias + o, sizeof(b));
+    else
 #pragma unroll
-    for (int r = 0; r < 4; r++)
-        if (o + r < p.n_out) v[r] += p.bias[o + r];
+        for (int r = 0; r < 4; r++) b[r] = p.bias[min(o + r, (long long)p.n_out - 1)];
+    return b;
 }
 // a lane's 32 outputs of row 16 t + c, block ob of 128, as the tile (t, ob) of the 8-bit form; what fills it up is 0
 __device__ __forceinline__ void store_held(const Fp8ProductParams &p, const Q8Shape &sy, long long t, long long ob, int lane, float (&v)[32])
@@ -353,16 +383,17 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
     }
 
     const long long ob = tw * WW + ww;                      // the wave's block of 128 outputs
+    f4 bias[FW];
+#pragma unroll
+    for (int n = 0; n < FW; n++) bias[n] = bias_of(p, 128 * ob + 16 * n + 4 * (lane >> 4));
 #pragma unroll
     for (int m = 0; m < FX; m++) {
         const long long t = tx * TX + wx * FX + m;
         float v[32];
 #pragma unroll
-        for (int n = 0; n < FW; n++) {
+        for (int n = 0; n < FW; n++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[4 * n + r] = acc[n][m][r];
-            add_bias(p, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
-        }
+            for (int r = 0; r < 4; r++) v[4 * n + r] = acc[n][m][r] + bias[n][r];
         activate(v, p.act);
         if (p.y_type == LCRC_T_E4M3) {
             if (t < sy.rt && ob < sy.kb) store_held(p, sy, t, ob, lane, v);
@@ -371,6 +402,138 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
             for (int n = 0; n < FW; n++) store_rows(p, 16 * t + c, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
         }
     }
+}
+
+// Few rows, or few results for a long sum: the waves of a workgroup share out the blocks of the sum, each for all of the
+// workgroup's 16 FW outputs x 16 FX rows, and the partial results are added up in LDS, in the waves' order.  Operands come
+// straight from memory.  X: rows of that type, which every wave converts for its own blocks (FX = 1), or unsigned char: rows
+// in the 8-bit form.
+template <bool EXACT, typename X, int FW, int FX, int NW>
+__global__ __launch_bounds__(64 * NW) void fp8_split_kernel(const Fp8ProductParams p, const void *x_rows, long long ldx)
+{
+    constexpr bool kRaw = sizeof(X) > 1;
+    static_assert(!kRaw || FX == 1, "one tile of rows is converted");
+    constexpr int U = FW <= 2 && sizeof(X) < 4 ? 2 : 1;     // blocks on their way at once (what the registers hold)
+    extern __shared__ __attribute__((aligned(16))) f4 parts[];           // [NW][FW * FX][64]
+    const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long w0 = (long long)blockIdx.x * FW, t0 = (long long)blockIdx.y * FX;
+    const X *row = kRaw ? static_cast<const X *>(x_rows) + (c < p.rows ? c : 0) * ldx : nullptr;
+    f4 acc[FW][FX];
+#pragma unroll
+    for (int n = 0; n < FW; n++)
+#pragma unroll
+        for (int m = 0; m < FX; m++) acc[n][m] = f4{0.f, 0.f, 0.f, 0.f};
+    for (long long k0 = wave; k0 < sx.kb; k0 += U * NW) {
+        i8 a[U][FW], b[U][FX];
+        int as[U][FW], bs[U][FX];
+        RawBlock<X> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long kb = min(k0 + u * NW, sx.kb - 1);
+#pragma unroll
+            for (int n = 0; n < FW; n++) {
+                const long long t = min(w0 + n, sw.rt - 1);
+                a[u][n] = load_tile(p.w + (t * sw.kb + kb) * kQTileBytes, lane);
+                as[u][n] = p.w[sw.scales_at() + ((t * sw.kb4 + (kb >> 2)) * 16 + c) * 4 + (kb & 3)];
+            }
+            if constexpr (kRaw) raw[u].load(row, kb, p.n_in, g);
+            else
+#pragma unroll
+                for (int m = 0; m < FX; m++) {
+                    const long long t = min(t0 + m, sx.rt - 1);
+                    b[u][m] = load_tile(p.x + (t * sx.kb + kb) * kQTileBytes, lane);
+                    bs[u][m] = p.x[sx.scales_at() + ((t * sx.kb4 + (kb >> 2)) * 16 + c) * 4 + (kb & 3)];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long kb = k0 + u * NW;
+            if (kb >= sx.kb) break;
+            if constexpr (kRaw) {
+                float v[32];
+                int e;
+                raw[u].values(v, c < p.rows, kb, p.n_in, g);
+                b[u][0] = quantise(v, &e);
+                bs[u][0] = e + 127;
+            }
+#pragma unroll
+            for (int n = 0; n < FW; n++)
+#pragma unroll
+                for (int m = 0; m < FX; m++) acc[n][m] = scaled_product<EXACT, 0>(a[u][n], b[u][m], acc[n][m], as[u][n], bs[u][m]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < FW; n++)
+#pragma unroll
+        for (int m = 0; m < FX; m++) parts[(wave * FW * FX + m * FW + n) * 64 + lane] = acc[n][m];
+    __syncthreads();
+    const auto total = [&](int tile) {
+        f4 v = parts[tile * 64 + lane];
+        for (int w = 1; w < NW; w++) v += parts[(w * FW * FX + tile) * 64 + lane];
+        return v;
+    };
+    if constexpr (FW == 8) {                                // whole blocks of outputs: the 8-bit form
+        if (wave >= FX) return;
+        float v[32];
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const f4 sum = total(wave * 8 + n) + bias_of(p, 16 * (w0 + n) + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[4 * n + r] = sum[r];
+        }
+        activate(v, p.act);
+        if (t0 + wave < sy.rt) store_held(p, sy, t0 + wave, blockIdx.x, lane, v);
+    } else {
+        for (int tile = wave; tile < FW * FX; tile += NW) {
+            const long long o = 16 * (w0 + tile % FW) + 4 * g;
+            const f4 sum = total(tile) + bias_of(p, o);
+            float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+            activate(v, p.act);
+            store_rows(p, 16 * (t0 + tile / FW) + c, o, v);
+        }
+    }
+}
+
+template <bool EXACT, typename X, int FW, int FX, int NW>
+void split_launch(const Fp8ProductParams &p, const void *x, long long ldx, hipStream_t stream)
+{
+    const dim3 grid((unsigned)(((long long)p.n_out + 16 * FW - 1) / (16 * FW)), (unsigned)(((long long)p.rows + 16 * FX - 1) / (16 * FX)));
+    fp8_split_kernel<EXACT, X, FW, FX, NW><<<grid, 64 * NW, NW * FW * FX * 1024, stream>>>(p, x, ldx);
+}
+template <bool EXACT, typename X>
+void split_launch(const Fp8ProductParams &p, const void *x, long long ldx, hipStream_t stream)
+{
+    const bool deep = p.n_in > 128 * 4;
+    if (p.y_type == LCRC_T_E4M3) {
+        if constexpr (!EXACT) {
+            if (deep) split_launch<EXACT, X, 8, 1, 8>(p, x, ldx, stream);
+            else split_launch<EXACT, X, 8, 1, 4>(p, x, ldx, stream);
+        }
+        return;
+    }
+    if constexpr (sizeof(X) == 1) {
+        if (p.rows > 32) {
+            if (deep) split_launch<EXACT, X, 1, 4, 16>(p, x, ldx, stream);
+            else split_launch<EXACT, X, 1, 4, 4>(p, x, ldx, stream);
+            return;
+        }
+        if (p.rows > 16) {
+            if (deep) split_launch<EXACT, X, 1, 2, 16>(p, x, ldx, stream);
+            else split_launch<EXACT, X, 1, 2, 4>(p, x, ldx, stream);
+            return;
+        }
+    }
+    if (!deep) split_launch<EXACT, X, 1, 1, 4>(p, x, ldx, stream);
+    else if (p.n_out >= 16 * 512) split_launch<EXACT, X, 2, 1, 16>(p, x, ldx, stream);
+    else split_launch<EXACT, X, 1, 1, 16>(p, x, ldx, stream);
+}
+template <typename X>
+hipError_t split_by_sums(const Fp8ProductParams &p, const void *x, long long ldx, hipStream_t stream)
+{
+    if (p.y_type == LCRC_T_F32) split_launch<true, X>(p, x, ldx, stream);
+    else split_launch<false, X>(p, x, ldx, stream);
+    return hipGetLastError();
 }
 
 template <bool EXACT, int FW, int FX, int WW, int WX>
@@ -415,6 +578,7 @@ hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream)
 
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
+    if (tiles(p, 128, 64) < 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
     if (p.y_type == LCRC_T_F32) {
         if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4>(p, stream);
         else tile_launch<true, 8, 1, 1, 4>(p, stream);
@@ -422,6 +586,13 @@ hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
     else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4>(p, stream);
     else tile_launch<false, 8, 1, 1, 4>(p, stream);
     return hipGetLastError();
+}
+
+hipError_t fp8_few_rows_launch(const Fp8ProductParams &p, const void *x, int x_type, long long ldx, hipStream_t stream)
+{
+    if (x_type == LCRC_T_F32) return split_by_sums<float>(p, x, ldx, stream);
+    if (x_type == LCRC_T_F16) return split_by_sums<_Float16>(p, x, ldx, stream);
+    return split_by_sums<__bf16>(p, x, ldx, stream);
 }
 
 }  // namespace phnrec

@@ -49,6 +49,15 @@ int check_rows(const char *call, const void *p, int type, int cols, long long ld
     return LCRC_OK;
 }
 
+// a matrix in the 8-bit form: the launches over its tiles stay within a grid
+int check_held(const char *call, const void *p, int rows, int cols)
+{
+    if (!p || !aligned(p, 16)) return bad(call, "an 8-bit matrix must be aligned to 16 bytes");
+    const Q8Shape s(rows, cols);
+    if (s.rt * s.kb > kQMaxTiles) return bad(call, "an 8-bit matrix of more than 2^26 tiles of 16 x 128");
+    return LCRC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -96,7 +105,7 @@ int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, 
     if ((type == LCRC_T_E4M3) != (scales != nullptr) && rows > 0) return bad(call, "scales belong to LCRC_T_E4M3 and to no other type");
     if (rows == 0) return LCRC_OK;
     if (const int rc = check_rows(call, src, type, cols, ld)) return rc;
-    if (!dst || !aligned(dst, 16)) return bad(call, "the 8-bit matrix must be aligned to 16 bytes");
+    if (const int rc = check_held(call, dst, rows, cols)) return rc;
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
     const Fp8PackParams p = {src, scales, type, rows, cols, ld, static_cast<unsigned char *>(dst)};
@@ -110,7 +119,7 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
     if (rows < 0 || cols < 1) return bad(call, "sizes: rows >= 0, cols >= 1");
     if (rows == 0) return LCRC_OK;
     if (const int rc = check_rows(call, dst, type, cols, ld)) return rc;
-    if (!src || !aligned(src, 16)) return bad(call, "the 8-bit matrix must be aligned to 16 bytes");
+    if (const int rc = check_held(call, src, rows, cols)) return rc;
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
     const Fp8UnpackParams p = {static_cast<const unsigned char *>(src), type, rows, cols, ld, dst};
@@ -128,15 +137,17 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     if (!a) return bad(call, "NULL argument");
     if (a->x_type < LCRC_T_F32 || a->x_type > LCRC_T_E4M3 || a->y_type < LCRC_T_F32 || a->y_type > LCRC_T_E4M3) return bad(call, "unknown type");
     if (a->act < LCRC_ACT_NONE || a->act > LCRC_ACT_FSIGMOID) return bad(call, "unknown activation");
-    if (a->rows < 0 || a->n_in < 1 || a->n_out < 1) return bad(call, "sizes: rows >= 0, n_in >= 1, n_out >= 1");
+    if (a->rows < 0 || a->n_in < 1 || a->n_in > kQMaxIn || a->n_out < 1) return bad(call, "sizes: rows >= 0, n_in 1 .. 2^23, n_out >= 1");
     if (a->rows == 0) return LCRC_OK;
     if (a->x_type == LCRC_T_E4M3) {
-        if (!a->x || !aligned(a->x, 16)) return bad(call, "an 8-bit matrix must be aligned to 16 bytes");
+        if (const int rc = check_held(call, a->x, a->rows, a->n_in)) return rc;
     } else if (const int rc = check_rows(call, a->x, a->x_type, a->n_in, a->ldx)) return rc;
     if (a->y_type == LCRC_T_E4M3) {
-        if (!a->y || !aligned(a->y, 16)) return bad(call, "an 8-bit matrix must be aligned to 16 bytes");
+        if (const int rc = check_held(call, a->y, a->rows, a->n_out)) return rc;
     } else if (const int rc = check_rows(call, a->y, a->y_type, a->n_out, a->ldy)) return rc;
-    if (!a->w || !aligned(a->w, 16)) return bad(call, "an 8-bit matrix must be aligned to 16 bytes");
+    if (const int rc = check_held(call, a->w, a->n_out, a->n_in)) return rc;
+    const Q8Shape sx(a->rows, a->n_in), sy(a->rows, a->n_out);
+    if (sx.rt * sx.kb > kQMaxTiles || sy.rt * sy.kb > kQMaxTiles) return bad(call, "x or y of more than 2^26 tiles of 16 x 128");
     if (!aligned(a->bias, 4)) return bad(call, "bias must be aligned to 4 bytes");
     const size_t need = lcrc_fp8_linear_workspace(a->rows, a->n_in, a->x_type);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)))
@@ -144,13 +155,14 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    const unsigned char *x = static_cast<const unsigned char *>(a->x);
+    const unsigned char *x = a->x_type == LCRC_T_E4M3 ? static_cast<const unsigned char *>(a->x) : nullptr;
+    Fp8ProductParams p = {x, static_cast<const unsigned char *>(a->w), a->bias, a->rows, a->n_in, a->n_out, a->act, a->y_type, a->y, a->ldy};
     if (a->x_type != LCRC_T_E4M3) {
-        const Fp8PackParams p = {a->x, nullptr, a->x_type, a->rows, a->n_in, a->ldx, static_cast<unsigned char *>(a->workspace)};
-        if (const int rc = launched(call, fp8_pack_launch(p, s))) return rc;
-        x = p.dst;
+        if (a->rows <= kQRows && a->n_out <= kQFewOut) return launched(call, fp8_few_rows_launch(p, a->x, a->x_type, a->ldx, s));
+        const Fp8PackParams pack = {a->x, nullptr, a->x_type, a->rows, a->n_in, a->ldx, static_cast<unsigned char *>(a->workspace)};
+        if (const int rc = launched(call, fp8_pack_launch(pack, s))) return rc;
+        p.x = pack.dst;
     }
-    const Fp8ProductParams p = {x, static_cast<const unsigned char *>(a->w), a->bias, a->rows, a->n_in, a->n_out, a->act, a->y_type, a->y, a->ldy};
     return launched(call, fp8_product_launch(p, s));
 }
 

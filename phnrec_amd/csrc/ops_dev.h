@@ -62,6 +62,11 @@ struct Fp8ProductParams {
 hipError_t fp8_pack_launch(const Fp8PackParams &p, hipStream_t stream);
 hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream);
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream);
+// up to kQRows rows of f32, f16 or bf16: converted by the product itself (p.x is not read)
+hipError_t fp8_few_rows_launch(const Fp8ProductParams &p, const void *x, int x_type, long long ldx, hipStream_t stream);
+constexpr int kQFewOut = 1 << 25;     // ... and up to this many outputs
+constexpr long long kQMaxTiles = 1ll << 26;      // of a matrix in the 8-bit form, of x and of y (a grid holds 2^32 threads)
+constexpr int kQMaxIn = 1 << 23;      // columns of the operands of a product: their tiles' offsets stay within 32 bits
 
 }  // namespace phnrec
 #endif
