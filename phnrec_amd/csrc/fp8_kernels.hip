@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "ops_dev.h"
 
@@ -292,8 +293,19 @@ __device__ __forceinline__ void store_held(const Fp8ProductParams &p, const Q8Sh
     if (ob == sy.kb - 1 && g > (ob & 3)) scales[g] = 127;
 }
 
-typedef const unsigned char __attribute__((address_space(1))) *global_bytes;
 typedef unsigned char __attribute__((address_space(3))) *lds_bytes;
+
+// N bytes for each lane from base + lane_offset + offset to the LDS, lane by lane, past the registers.  (As a buffer load: with
+// one on its way, a wait for LDS reads that were asked for before it need not become a wait for all of them.)
+template <int N>
+__device__ __forceinline__ void copy_to_lds(const unsigned char *base, unsigned lane_offset, int offset, unsigned char *to)
+{
+#ifdef __HIP_DEVICE_COMPILE__               // (the host has no such type)
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, -1, 0x00027000);
+    if constexpr (N == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_bytes)to, 16, lane_offset, offset, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_bytes)to, 4, lane_offset, offset, 0, 0);
+#endif
+}
 
 // block J of a group of four, scale bytes J of the groups' dwords
 template <bool EXACT, int J>
@@ -303,13 +315,21 @@ __device__ __forceinline__ f4 scaled_product(const i8 &a, const i8 &b, f4 acc, i
     else return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, J, as, J, bs);
 }
 
+template <typename F, int... M>
+__device__ __forceinline__ void for_each(const F &f, std::integer_sequence<int, M...>)
+{
+    (f(std::integral_constant<int, M>()), ...);
+}
+
 // A workgroup of WW x WX waves makes 16 FW WW outputs of 16 FX WX rows, each wave FW x FX tiles in its registers.
-template <bool EXACT, int FW, int FX, int WW, int WX>
-__global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
+template <bool EXACT, int FW, int FX, int WW, int WX, int STAGES = 1>
+__global__ __launch_bounds__(64 * WW * WX, FX == 8 ? 1 : 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
 {
     constexpr int kWaves = WW * WX, TW = FW * WW, TX = FX * WX, PW = 2 * TW / kWaves, PX = 2 * TX / kWaves, kPiece = kQTileBytes / 2;
     static_assert(FW == 8 && PW * kWaves == 2 * TW && PX * kWaves == 2 * TX, "whole blocks of outputs; the copies are shared out evenly");
-    __shared__ __attribute__((aligned(16))) unsigned char stage[(TW + TX) * kQTileBytes];
+    constexpr int kStage = (TW + TX) * kQTileBytes;
+    __shared__ __attribute__((aligned(16))) unsigned char stages[STAGES * kStage];
+    __shared__ __attribute__((aligned(16))) unsigned char scale_stages[2 * (TW + TX) * 64];
     const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
     const int lane = threadIdx.x & 63, c = lane & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ww = wave % WW, wx = wave / WW;
@@ -331,63 +351,79 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
     for (int q = 0; q < PW; q++) wp[q] = min((wave * PW + q) >> 1, w_left) * tile_stride + (q & 1) * kPiece + lane * 16;
 #pragma unroll
     for (int q = 0; q < PX; q++) xp[q] = min((wave * PX + q) >> 1, x_left) * tile_stride + (q & 1) * kPiece + lane * 16;
-    const auto fetch = [&](long long kb) {                  // block kb of the operands into the stage, past the registers
+    const auto fetch = [&](int kb, int to) {                // block kb of the operands into a stage, past the registers
+        unsigned char *const stage = stages + (STAGES > 1 ? to * kStage : 0);
 #pragma unroll
-        for (int q = 0; q < PW; q++)
-            __builtin_amdgcn_global_load_lds((global_bytes)(w0 + kb * kQTileBytes + wp[q]), (lds_bytes)(stage + (wave * PW + q) * kPiece), 16, 0, 0);
+        for (int q = 0; q < PW; q++) copy_to_lds<16>(w0, wp[q], kb * kQTileBytes, stage + (wave * PW + q) * kPiece);
 #pragma unroll
-        for (int q = 0; q < PX; q++)
-            __builtin_amdgcn_global_load_lds((global_bytes)(x0 + kb * kQTileBytes + xp[q]), (lds_bytes)(stage + (2 * TW + wave * PX + q) * kPiece), 16, 0, 0);
+        for (int q = 0; q < PX; q++) copy_to_lds<16>(x0, xp[q], kb * kQTileBytes, stage + (2 * TW + wave * PX + q) * kPiece);
     };
     const unsigned char *const ws = p.w + sw.scales_at() + tw * TW * sw.kb4 * 64, *const xs = p.x + sx.scales_at() + tx * TX * sx.kb4 * 64;
-    int s[FW + FX];
-    const auto fetch_scales = [&](long long kb4) {          // of four blocks: a dword for each row
+    const auto fetch_scales = [&](int kb4) {                // of four blocks: a dword for each row, four tiles to a copy
 #pragma unroll
-        for (int n = 0; n < FW; n++)
-            s[n] = *reinterpret_cast<const int *>(ws + kb4 * 64 + min(ww * FW + n, w_left) * scale_stride + c * 4);
-#pragma unroll
-        for (int n = 0; n < FX; n++)
-            s[FW + n] = *reinterpret_cast<const int *>(xs + kb4 * 64 + min(wx * FX + n, x_left) * scale_stride + c * 4);
+        for (int q = 0; q < (TW + TX) / 4; q++) {
+            const int tile = 4 * q + (lane >> 4);
+            if (q % kWaves != wave) continue;
+            const unsigned at = (4 * q < TW ? min(tile, w_left) : min(tile - TW, x_left)) * scale_stride + c * 4;
+            copy_to_lds<4>(4 * q < TW ? ws : xs, at, kb4 * 64, scale_stages + (kb4 & 1) * (TW + TX) * 64 + q * 256);
+        }
     };
+    int s[FW + FX];
 
     f4 acc[FW][FX];
 #pragma unroll
     for (int n = 0; n < FW; n++)
 #pragma unroll
         for (int m = 0; m < FX; m++) acc[n][m] = f4{0.f, 0.f, 0.f, 0.f};
-    const auto step = [&](long long kb, auto j) {
+    const int blocks = (int)sx.kb;
+    const auto step = [&](int kb, auto j) {
         constexpr int J = decltype(j)::value;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's copies have arrived (a barrier alone does not wait for them)
         __syncthreads();                                    // ... and everyone's
+        const unsigned char *const stage = stages + (STAGES > 1 ? (J & 1) * kStage : 0);
+        if constexpr (J == 0) {
+            const int *const rows = reinterpret_cast<const int *>(scale_stages + (kb >> 2 & 1) * (TW + TX) * 64) + c;
+#pragma unroll
+            for (int n = 0; n < FW; n++) s[n] = rows[16 * (ww * FW + n)];
+#pragma unroll
+            for (int m = 0; m < FX; m++) s[FW + m] = rows[16 * (TW + wx * FX + m)];
+        }
         i8 a[FW], b[FX];
+        a[0] = load_tile(stage + ww * FW * kQTileBytes, lane);
 #pragma unroll
         for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
 #pragma unroll
-        for (int n = 0; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                       // ... and read by all
-        if (kb + 1 < sx.kb) fetch(kb + 1);                  // on its way while the products run
+        for (int n = 1; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
+        if constexpr (STAGES == 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                   // ... and read by all
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // on its way while the products run (behind the last block: that one again, without a branch around the copies)
+        fetch(min(kb + 1, blocks - 1), (J + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < FW; n++)
 #pragma unroll
             for (int m = 0; m < FX; m++) acc[n][m] = scaled_product<EXACT, J>(a[n], b[m], acc[n][m], s[n], s[FW + m]);
     };
-    fetch(0);
+    fetch(0, 0);
     fetch_scales(0);
-    for (long long kb = 0; kb < sx.kb; kb += 4) {
+    for (int kb = 0; kb < blocks; kb += 4) {
         step(kb, std::integral_constant<int, 0>());
-        if (kb + 1 < sx.kb) step(kb + 1, std::integral_constant<int, 1>());
-        if (kb + 2 < sx.kb) step(kb + 2, std::integral_constant<int, 2>());
-        if (kb + 3 < sx.kb) step(kb + 3, std::integral_constant<int, 3>());
-        if (kb + 4 < sx.kb) fetch_scales(kb / 4 + 1);
+        if (kb + 4 < blocks) fetch_scales(kb / 4 + 1);
+        if (kb + 1 < blocks) step(kb + 1, std::integral_constant<int, 1>());
+        if (kb + 2 < blocks) step(kb + 2, std::integral_constant<int, 2>());
+        if (kb + 3 < blocks) step(kb + 3, std::integral_constant<int, 3>());
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // (no copy outlives the workgroup's LDS)
 
     const long long ob = tw * WW + ww;                      // the wave's block of 128 outputs
     f4 bias[FW];
 #pragma unroll
     for (int n = 0; n < FW; n++) bias[n] = bias_of(p, 128 * ob + 16 * n + 4 * (lane >> 4));
-#pragma unroll
-    for (int m = 0; m < FX; m++) {
+    const auto finish = [&](auto which) {
+        constexpr int m = decltype(which)::value;
         const long long t = tx * TX + wx * FX + m;
         float v[32];
 #pragma unroll
@@ -401,7 +437,9 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
 #pragma unroll
             for (int n = 0; n < FW; n++) store_rows(p, 16 * t + c, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
         }
-    }
+    };
+    // (spelled out: an accumulator with an index that is not known when compiling would leave the registers)
+    for_each(finish, std::make_integer_sequence<int, FX>());
 }
 
 // Few rows, or few results for a long sum: the waves of a workgroup share out the blocks of the sum, each for all of the
@@ -536,12 +574,12 @@ hipError_t split_by_sums(const Fp8ProductParams &p, const void *x, long long ldx
     return hipGetLastError();
 }
 
-template <bool EXACT, int FW, int FX, int WW, int WX>
+template <bool EXACT, int FW, int FX, int WW, int WX, int STAGES = 1>
 void tile_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
     const long long across = ((long long)p.n_out + 16 * FW * WW - 1) / (16 * FW * WW), down = ((long long)p.rows + 16 * FX * WX - 1) / (16 * FX * WX);
     const long long blocks = (across * down + 7) / 8 * 8;
-    fp8_tile_kernel<EXACT, FW, FX, WW, WX><<<(unsigned)blocks, 64 * WW * WX, 0, stream>>>(p, (int)across, (int)down);
+    fp8_tile_kernel<EXACT, FW, FX, WW, WX, STAGES><<<(unsigned)blocks, 64 * WW * WX, 0, stream>>>(p, (int)across, (int)down);
 }
 // tiles of 16 FW WW outputs x 16 FX WX rows
 long long tiles(const Fp8ProductParams &p, int outputs, int rows)
@@ -582,7 +620,8 @@ hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
     if (p.y_type == LCRC_T_F32) {
         if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4>(p, stream);
         else tile_launch<true, 8, 1, 1, 4>(p, stream);
-    } else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
+    } else if (tiles(p, 256, 256) >= 256) tile_launch<false, 8, 8, 2, 2, 2>(p, stream);
+    else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
     else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4>(p, stream);
     else tile_launch<false, 8, 1, 1, 4>(p, stream);
     return hipGetLastError();
