@@ -266,6 +266,47 @@ __device__ __forceinline__ void store_rows(const Fp8ProductParams &p, long long 
     else if (p.y_type == LCRC_T_F16) store_four(static_cast<_Float16 *>(p.y) + row * p.ldy, o, p.n_out, v);
     else store_four(static_cast<__bf16 *>(p.y) + row * p.ldy, o, p.n_out, v);
 }
+// A lane's 32 outputs o .. o + 127 of rows row0 .. row0 + 15, turned in LDS (`turn`, this wave's own) so that 16 lanes write
+// 256 consecutive bytes of a row: written as they lie in the registers, 32 bytes of a row at a time, they cost 2 to 3 times
+// as long.  (Rows of 288 bytes in LDS: eight lanes' writes of 8 bytes meet no bank twice.)
+constexpr int kTurnRow = 256 + 32, kTurn = 16 * kTurnRow;
+template <typename Y>
+__device__ __forceinline__ void store_block(const Fp8ProductParams &p, long long row0, long long o, int lane, const float (&v)[32], unsigned char *turn)
+{
+    constexpr int kOutputs = 256 / sizeof(Y), E = 16 / sizeof(Y);
+    struct Four { Y v[4]; };
+    struct Chunk { Y v[E]; };
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < 128 / kOutputs; half++) {
+#pragma unroll
+        for (int n = 0; n < kOutputs / 16; n++) {
+            const float *f = v + 4 * (half * (kOutputs / 16) + n);
+            const Four q = {{(Y)f[0], (Y)f[1], (Y)f[2], (Y)f[3]}};
+            __builtin_memcpy(__builtin_assume_aligned(turn + c * kTurnRow + (16 * n + 4 * g) * (int)sizeof(Y), 8), &q, sizeof(q));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const long long at = o + half * kOutputs + c * E;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 4 * i + g;
+            Chunk q;
+            __builtin_memcpy(&q, __builtin_assume_aligned(turn + r * kTurnRow + c * 16, 16), 16);
+            if (row0 + r >= p.rows) continue;
+            Y *y = static_cast<Y *>(p.y) + (row0 + r) * p.ldy + at;
+            if (at + E <= p.n_out) __builtin_memcpy(y, &q, 16);
+            else
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (at + e < p.n_out) y[e] = q.v[e];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
 // the bias of outputs o .. o + 3 (0 without one; what lies behind the last output is not used)
 __device__ __forceinline__ f4 bias_of(const Fp8ProductParams &p, long long o)
 {
@@ -307,6 +348,99 @@ __device__ __forceinline__ void copy_to_lds(const unsigned char *base, unsigned 
 #endif
 }
 
+// s_waitcnt's operand: vmcnt(vm) lgkmcnt(lgkm)
+constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }
+
+// A wave's tiles of a stage (w: those of W, x: those of x, each 2048 bytes behind the one before) and their scales, with the
+// wait for them.  Written out, because the compiler waits for ALL copies to LDS before a read of LDS that it knows of, also
+// for those of later blocks.
+__device__ __forceinline__ unsigned lds_address(const unsigned char *p)
+{
+    return (unsigned)(uintptr_t)(lds_bytes) const_cast<unsigned char *>(p);
+}
+__device__ __forceinline__ void read_tiles(const unsigned char *w, const unsigned char *x, int lane, i8 (&a)[8], i8 (&b)[1])
+{
+    i4 l[9], h[9];
+    asm volatile(
+                 "ds_read_b128 %0, %18 offset:0\n ds_read_b128 %9, %18 offset:1024\n"
+                 "ds_read_b128 %1, %18 offset:2048\n ds_read_b128 %10, %18 offset:3072\n"
+                 "ds_read_b128 %2, %18 offset:4096\n ds_read_b128 %11, %18 offset:5120\n"
+                 "ds_read_b128 %3, %18 offset:6144\n ds_read_b128 %12, %18 offset:7168\n"
+                 "ds_read_b128 %4, %18 offset:8192\n ds_read_b128 %13, %18 offset:9216\n"
+                 "ds_read_b128 %5, %18 offset:10240\n ds_read_b128 %14, %18 offset:11264\n"
+                 "ds_read_b128 %6, %18 offset:12288\n ds_read_b128 %15, %18 offset:13312\n"
+                 "ds_read_b128 %7, %18 offset:14336\n ds_read_b128 %16, %18 offset:15360\n"
+                 "ds_read_b128 %8, %19 offset:0\n ds_read_b128 %17, %19 offset:1024\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(l[4]), "=&v"(l[5]), "=&v"(l[6]), "=&v"(l[7]), "=&v"(l[8]),
+                   "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7]), "=&v"(h[8])
+                 : "v"(lds_address(w) + lane * 16), "v"(lds_address(x) + lane * 16)
+                 : "memory");
+#pragma unroll
+    for (int n = 0; n < 8; n++) a[n] = __builtin_shufflevector(l[n], h[n], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int m = 0; m < 1; m++) b[m] = __builtin_shufflevector(l[8 + m], h[8 + m], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ void read_tiles(const unsigned char *w, const unsigned char *x, int lane, i8 (&a)[8], i8 (&b)[2])
+{
+    i4 l[10], h[10];
+    asm volatile(
+                 "ds_read_b128 %0, %20 offset:0\n ds_read_b128 %10, %20 offset:1024\n"
+                 "ds_read_b128 %1, %20 offset:2048\n ds_read_b128 %11, %20 offset:3072\n"
+                 "ds_read_b128 %2, %20 offset:4096\n ds_read_b128 %12, %20 offset:5120\n"
+                 "ds_read_b128 %3, %20 offset:6144\n ds_read_b128 %13, %20 offset:7168\n"
+                 "ds_read_b128 %4, %20 offset:8192\n ds_read_b128 %14, %20 offset:9216\n"
+                 "ds_read_b128 %5, %20 offset:10240\n ds_read_b128 %15, %20 offset:11264\n"
+                 "ds_read_b128 %6, %20 offset:12288\n ds_read_b128 %16, %20 offset:13312\n"
+                 "ds_read_b128 %7, %20 offset:14336\n ds_read_b128 %17, %20 offset:15360\n"
+                 "ds_read_b128 %8, %21 offset:0\n ds_read_b128 %18, %21 offset:1024\n"
+                 "ds_read_b128 %9, %21 offset:2048\n ds_read_b128 %19, %21 offset:3072\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(l[4]), "=&v"(l[5]), "=&v"(l[6]), "=&v"(l[7]), "=&v"(l[8]), "=&v"(l[9]),
+                   "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7]), "=&v"(h[8]), "=&v"(h[9])
+                 : "v"(lds_address(w) + lane * 16), "v"(lds_address(x) + lane * 16)
+                 : "memory");
+#pragma unroll
+    for (int n = 0; n < 8; n++) a[n] = __builtin_shufflevector(l[n], h[n], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int m = 0; m < 2; m++) b[m] = __builtin_shufflevector(l[8 + m], h[8 + m], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ void read_scales(const unsigned char *w, const unsigned char *x, int c, int (&s)[9])
+{
+    asm volatile(
+                 "ds_read_b32 %0, %9 offset:0\n"
+                 "ds_read_b32 %1, %9 offset:64\n"
+                 "ds_read_b32 %2, %9 offset:128\n"
+                 "ds_read_b32 %3, %9 offset:192\n"
+                 "ds_read_b32 %4, %9 offset:256\n"
+                 "ds_read_b32 %5, %9 offset:320\n"
+                 "ds_read_b32 %6, %9 offset:384\n"
+                 "ds_read_b32 %7, %9 offset:448\n"
+                 "ds_read_b32 %8, %10 offset:0\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(s[4]), "=&v"(s[5]), "=&v"(s[6]), "=&v"(s[7]), "=&v"(s[8])
+                 : "v"(lds_address(w) + c * 4), "v"(lds_address(x) + c * 4)
+                 : "memory");
+}
+__device__ __forceinline__ void read_scales(const unsigned char *w, const unsigned char *x, int c, int (&s)[10])
+{
+    asm volatile(
+                 "ds_read_b32 %0, %10 offset:0\n"
+                 "ds_read_b32 %1, %10 offset:64\n"
+                 "ds_read_b32 %2, %10 offset:128\n"
+                 "ds_read_b32 %3, %10 offset:192\n"
+                 "ds_read_b32 %4, %10 offset:256\n"
+                 "ds_read_b32 %5, %10 offset:320\n"
+                 "ds_read_b32 %6, %10 offset:384\n"
+                 "ds_read_b32 %7, %10 offset:448\n"
+                 "ds_read_b32 %8, %11 offset:0\n"
+                 "ds_read_b32 %9, %11 offset:64\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(s[4]), "=&v"(s[5]), "=&v"(s[6]), "=&v"(s[7]), "=&v"(s[8]), "=&v"(s[9])
+                 : "v"(lds_address(w) + c * 4), "v"(lds_address(x) + c * 4)
+                 : "memory");
+}
+
 // block J of a group of four, scale bytes J of the groups' dwords
 template <bool EXACT, int J>
 __device__ __forceinline__ f4 scaled_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
@@ -323,11 +457,11 @@ __device__ __forceinline__ void for_each(const F &f, std::integer_sequence<int, 
 
 // A workgroup of WW x WX waves makes 16 FW WW outputs of 16 FX WX rows, each wave FW x FX tiles in its registers.
 template <bool EXACT, int FW, int FX, int WW, int WX, int STAGES = 1>
-__global__ __launch_bounds__(64 * WW * WX, FX == 8 ? 1 : 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
+__global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
 {
     constexpr int kWaves = WW * WX, TW = FW * WW, TX = FX * WX, PW = 2 * TW / kWaves, PX = 2 * TX / kWaves, kPiece = kQTileBytes / 2;
     static_assert(FW == 8 && PW * kWaves == 2 * TW && PX * kWaves == 2 * TX, "whole blocks of outputs; the copies are shared out evenly");
-    constexpr int kStage = (TW + TX) * kQTileBytes;
+    constexpr int kStage = (TW + TX) * kQTileBytes, kAhead = STAGES > 1 ? STAGES - 1 : 1;
     __shared__ __attribute__((aligned(16))) unsigned char stages[STAGES * kStage];
     __shared__ __attribute__((aligned(16))) unsigned char scale_stages[2 * (TW + TX) * 64];
     const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
@@ -378,37 +512,50 @@ __global__ __launch_bounds__(64 * WW * WX, FX == 8 ? 1 : 2) void fp8_tile_kernel
     const int blocks = (int)sx.kb;
     const auto step = [&](int kb, auto j) {
         constexpr int J = decltype(j)::value;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's copies have arrived (a barrier alone does not wait for them)
-        __syncthreads();                                    // ... and everyone's
-        const unsigned char *const stage = stages + (STAGES > 1 ? (J & 1) * kStage : 0);
+        // this wave's copies of the block have arrived (a barrier alone does not wait for them; later blocks' may be on their way)
+        // and its reads of the block before are done
+        __builtin_amdgcn_s_waitcnt(wait_for(STAGES > 2 ? (STAGES - 2) * (PW + PX) : 0, 0));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();                       // ... and everyone's
+        asm volatile("" ::: "memory");
+        const unsigned char *const stage = stages + (STAGES > 1 ? kb % STAGES * kStage : 0);
         if constexpr (J == 0) {
-            const int *const rows = reinterpret_cast<const int *>(scale_stages + (kb >> 2 & 1) * (TW + TX) * 64) + c;
+            const unsigned char *const rows = scale_stages + (kb >> 2 & 1) * (TW + TX) * 64;
+            if constexpr (STAGES == 1) {
 #pragma unroll
-            for (int n = 0; n < FW; n++) s[n] = rows[16 * (ww * FW + n)];
+                for (int n = 0; n < FW; n++) s[n] = reinterpret_cast<const int *>(rows)[16 * (ww * FW + n) + c];
 #pragma unroll
-            for (int m = 0; m < FX; m++) s[FW + m] = rows[16 * (TW + wx * FX + m)];
+                for (int m = 0; m < FX; m++) s[FW + m] = reinterpret_cast<const int *>(rows)[16 * (TW + wx * FX + m) + c];
+            } else {
+                read_scales(rows + 64 * ww * FW, rows + 64 * (TW + wx * FX), c, s);
+            }
         }
         i8 a[FW], b[FX];
-        a[0] = load_tile(stage + ww * FW * kQTileBytes, lane);
+        if constexpr (STAGES == 1) {
+            a[0] = load_tile(stage + ww * FW * kQTileBytes, lane);
 #pragma unroll
-        for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
+            for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
 #pragma unroll
-        for (int n = 1; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
+            for (int n = 1; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
+        } else {
+            read_tiles(stage + ww * FW * kQTileBytes, stage + (TW + wx * FX) * kQTileBytes, lane, a, b);
+        }
         if constexpr (STAGES == 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                   // ... and read by all
         }
         __builtin_amdgcn_sched_barrier(0);
         // on its way while the products run (behind the last block: that one again, without a branch around the copies)
-        fetch(min(kb + 1, blocks - 1), (J + 1) & 1);
+        fetch(min(kb + kAhead, blocks - 1), (kb + kAhead) % STAGES);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < FW; n++)
 #pragma unroll
             for (int m = 0; m < FX; m++) acc[n][m] = scaled_product<EXACT, J>(a[n], b[m], acc[n][m], s[n], s[FW + m]);
     };
-    fetch(0, 0);
     fetch_scales(0);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) fetch(min(k, blocks - 1), k);
     for (int kb = 0; kb < blocks; kb += 4) {
         step(kb, std::integral_constant<int, 0>());
         if (kb + 4 < blocks) fetch_scales(kb / 4 + 1);
@@ -433,11 +580,12 @@ __global__ __launch_bounds__(64 * WW * WX, FX == 8 ? 1 : 2) void fp8_tile_kernel
         activate(v, p.act);
         if (p.y_type == LCRC_T_E4M3) {
             if (t < sy.rt && ob < sy.kb) store_held(p, sy, t, ob, lane, v);
-        } else {
-#pragma unroll
-            for (int n = 0; n < FW; n++) store_rows(p, 16 * t + c, 128 * ob + 16 * n + 4 * (lane >> 4), v + 4 * n);
-        }
+        } else if (p.y_type == LCRC_T_F32) store_block<float>(p, 16 * t, 128 * ob, lane, v, stages + wave * kTurn);
+        else if (p.y_type == LCRC_T_F16) store_block<_Float16>(p, 16 * t, 128 * ob, lane, v, stages + wave * kTurn);
+        else store_block<__bf16>(p, 16 * t, 128 * ob, lane, v, stages + wave * kTurn);
     };
+    static_assert(kWaves * kTurn <= STAGES * kStage, "the stages hold the turned results");
+    __syncthreads();                                        // the stages are read
     // (spelled out: an accumulator with an index that is not known when compiling would leave the registers)
     for_each(finish, std::make_integer_sequence<int, FX>());
 }
@@ -618,12 +766,11 @@ hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
     if (tiles(p, 128, 64) < 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
     if (p.y_type == LCRC_T_F32) {
-        if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4>(p, stream);
-        else tile_launch<true, 8, 1, 1, 4>(p, stream);
-    } else if (tiles(p, 256, 256) >= 256) tile_launch<false, 8, 8, 2, 2, 2>(p, stream);
-    else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
-    else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4>(p, stream);
-    else tile_launch<false, 8, 1, 1, 4>(p, stream);
+        if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4, 2>(p, stream);
+        else tile_launch<true, 8, 1, 1, 4, 3>(p, stream);
+    } else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
+    else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4, 2>(p, stream);
+    else tile_launch<false, 8, 1, 1, 4, 3>(p, stream);
     return hipGetLastError();
 }
 
