@@ -348,99 +348,6 @@ __device__ __forceinline__ void copy_to_lds(const unsigned char *base, unsigned 
 #endif
 }
 
-// s_waitcnt's operand: vmcnt(vm) lgkmcnt(lgkm)
-constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | lgkm << 8; }
-
-// A wave's tiles of a stage (w: those of W, x: those of x, each 2048 bytes behind the one before) and their scales, with the
-// wait for them.  Written out, because the compiler waits for ALL copies to LDS before a read of LDS that it knows of, also
-// for those of later blocks.
-__device__ __forceinline__ unsigned lds_address(const unsigned char *p)
-{
-    return (unsigned)(uintptr_t)(lds_bytes) const_cast<unsigned char *>(p);
-}
-__device__ __forceinline__ void read_tiles(const unsigned char *w, const unsigned char *x, int lane, i8 (&a)[8], i8 (&b)[1])
-{
-    i4 l[9], h[9];
-    asm volatile(
-                 "ds_read_b128 %0, %18 offset:0\n ds_read_b128 %9, %18 offset:1024\n"
-                 "ds_read_b128 %1, %18 offset:2048\n ds_read_b128 %10, %18 offset:3072\n"
-                 "ds_read_b128 %2, %18 offset:4096\n ds_read_b128 %11, %18 offset:5120\n"
-                 "ds_read_b128 %3, %18 offset:6144\n ds_read_b128 %12, %18 offset:7168\n"
-                 "ds_read_b128 %4, %18 offset:8192\n ds_read_b128 %13, %18 offset:9216\n"
-                 "ds_read_b128 %5, %18 offset:10240\n ds_read_b128 %14, %18 offset:11264\n"
-                 "ds_read_b128 %6, %18 offset:12288\n ds_read_b128 %15, %18 offset:13312\n"
-                 "ds_read_b128 %7, %18 offset:14336\n ds_read_b128 %16, %18 offset:15360\n"
-                 "ds_read_b128 %8, %19 offset:0\n ds_read_b128 %17, %19 offset:1024\n"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(l[4]), "=&v"(l[5]), "=&v"(l[6]), "=&v"(l[7]), "=&v"(l[8]),
-                   "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7]), "=&v"(h[8])
-                 : "v"(lds_address(w) + lane * 16), "v"(lds_address(x) + lane * 16)
-                 : "memory");
-#pragma unroll
-    for (int n = 0; n < 8; n++) a[n] = __builtin_shufflevector(l[n], h[n], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int m = 0; m < 1; m++) b[m] = __builtin_shufflevector(l[8 + m], h[8 + m], 0, 1, 2, 3, 4, 5, 6, 7);
-}
-__device__ __forceinline__ void read_tiles(const unsigned char *w, const unsigned char *x, int lane, i8 (&a)[8], i8 (&b)[2])
-{
-    i4 l[10], h[10];
-    asm volatile(
-                 "ds_read_b128 %0, %20 offset:0\n ds_read_b128 %10, %20 offset:1024\n"
-                 "ds_read_b128 %1, %20 offset:2048\n ds_read_b128 %11, %20 offset:3072\n"
-                 "ds_read_b128 %2, %20 offset:4096\n ds_read_b128 %12, %20 offset:5120\n"
-                 "ds_read_b128 %3, %20 offset:6144\n ds_read_b128 %13, %20 offset:7168\n"
-                 "ds_read_b128 %4, %20 offset:8192\n ds_read_b128 %14, %20 offset:9216\n"
-                 "ds_read_b128 %5, %20 offset:10240\n ds_read_b128 %15, %20 offset:11264\n"
-                 "ds_read_b128 %6, %20 offset:12288\n ds_read_b128 %16, %20 offset:13312\n"
-                 "ds_read_b128 %7, %20 offset:14336\n ds_read_b128 %17, %20 offset:15360\n"
-                 "ds_read_b128 %8, %21 offset:0\n ds_read_b128 %18, %21 offset:1024\n"
-                 "ds_read_b128 %9, %21 offset:2048\n ds_read_b128 %19, %21 offset:3072\n"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(l[4]), "=&v"(l[5]), "=&v"(l[6]), "=&v"(l[7]), "=&v"(l[8]), "=&v"(l[9]),
-                   "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7]), "=&v"(h[8]), "=&v"(h[9])
-                 : "v"(lds_address(w) + lane * 16), "v"(lds_address(x) + lane * 16)
-                 : "memory");
-#pragma unroll
-    for (int n = 0; n < 8; n++) a[n] = __builtin_shufflevector(l[n], h[n], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int m = 0; m < 2; m++) b[m] = __builtin_shufflevector(l[8 + m], h[8 + m], 0, 1, 2, 3, 4, 5, 6, 7);
-}
-__device__ __forceinline__ void read_scales(const unsigned char *w, const unsigned char *x, int c, int (&s)[9])
-{
-    asm volatile(
-                 "ds_read_b32 %0, %9 offset:0\n"
-                 "ds_read_b32 %1, %9 offset:64\n"
-                 "ds_read_b32 %2, %9 offset:128\n"
-                 "ds_read_b32 %3, %9 offset:192\n"
-                 "ds_read_b32 %4, %9 offset:256\n"
-                 "ds_read_b32 %5, %9 offset:320\n"
-                 "ds_read_b32 %6, %9 offset:384\n"
-                 "ds_read_b32 %7, %9 offset:448\n"
-                 "ds_read_b32 %8, %10 offset:0\n"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(s[4]), "=&v"(s[5]), "=&v"(s[6]), "=&v"(s[7]), "=&v"(s[8])
-                 : "v"(lds_address(w) + c * 4), "v"(lds_address(x) + c * 4)
-                 : "memory");
-}
-__device__ __forceinline__ void read_scales(const unsigned char *w, const unsigned char *x, int c, int (&s)[10])
-{
-    asm volatile(
-                 "ds_read_b32 %0, %10 offset:0\n"
-                 "ds_read_b32 %1, %10 offset:64\n"
-                 "ds_read_b32 %2, %10 offset:128\n"
-                 "ds_read_b32 %3, %10 offset:192\n"
-                 "ds_read_b32 %4, %10 offset:256\n"
-                 "ds_read_b32 %5, %10 offset:320\n"
-                 "ds_read_b32 %6, %10 offset:384\n"
-                 "ds_read_b32 %7, %10 offset:448\n"
-                 "ds_read_b32 %8, %11 offset:0\n"
-                 "ds_read_b32 %9, %11 offset:64\n"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3]), "=&v"(s[4]), "=&v"(s[5]), "=&v"(s[6]), "=&v"(s[7]), "=&v"(s[8]), "=&v"(s[9])
-                 : "v"(lds_address(w) + c * 4), "v"(lds_address(x) + c * 4)
-                 : "memory");
-}
-
 // block J of a group of four, scale bytes J of the groups' dwords
 template <bool EXACT, int J>
 __device__ __forceinline__ f4 scaled_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
@@ -461,7 +368,7 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
 {
     constexpr int kWaves = WW * WX, TW = FW * WW, TX = FX * WX, PW = 2 * TW / kWaves, PX = 2 * TX / kWaves, kPiece = kQTileBytes / 2;
     static_assert(FW == 8 && PW * kWaves == 2 * TW && PX * kWaves == 2 * TX, "whole blocks of outputs; the copies are shared out evenly");
-    constexpr int kStage = (TW + TX) * kQTileBytes, kAhead = STAGES > 1 ? STAGES - 1 : 1;
+    constexpr int kStage = (TW + TX) * kQTileBytes;
     __shared__ __attribute__((aligned(16))) unsigned char stages[STAGES * kStage];
     __shared__ __attribute__((aligned(16))) unsigned char scale_stages[2 * (TW + TX) * 64];
     const Q8Shape sx(p.rows, p.n_in), sw(p.n_out, p.n_in), sy(p.rows, p.n_out);
@@ -486,7 +393,7 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
 #pragma unroll
     for (int q = 0; q < PX; q++) xp[q] = min((wave * PX + q) >> 1, x_left) * tile_stride + (q & 1) * kPiece + lane * 16;
     const auto fetch = [&](int kb, int to) {                // block kb of the operands into a stage, past the registers
-        unsigned char *const stage = stages + (STAGES > 1 ? to * kStage : 0);
+        unsigned char *const stage = stages + to * kStage;
 #pragma unroll
         for (int q = 0; q < PW; q++) copy_to_lds<16>(w0, wp[q], kb * kQTileBytes, stage + (wave * PW + q) * kPiece);
 #pragma unroll
@@ -512,41 +419,31 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
     const int blocks = (int)sx.kb;
     const auto step = [&](int kb, auto j) {
         constexpr int J = decltype(j)::value;
-        // this wave's copies of the block have arrived (a barrier alone does not wait for them; later blocks' may be on their way)
-        // and its reads of the block before are done
-        __builtin_amdgcn_s_waitcnt(wait_for(STAGES > 2 ? (STAGES - 2) * (PW + PX) : 0, 0));
-        asm volatile("" ::: "memory");
+        // this wave's copies of the block have arrived (a barrier alone does not wait for them), its reads of the one before are done
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                       // ... and everyone's
         asm volatile("" ::: "memory");
-        const unsigned char *const stage = stages + (STAGES > 1 ? kb % STAGES * kStage : 0);
+        const unsigned char *const stage = stages + (kb % STAGES) * kStage;
         if constexpr (J == 0) {
-            const unsigned char *const rows = scale_stages + (kb >> 2 & 1) * (TW + TX) * 64;
-            if constexpr (STAGES == 1) {
+            const int *const rows = reinterpret_cast<const int *>(scale_stages + (kb >> 2 & 1) * (TW + TX) * 64) + c;
 #pragma unroll
-                for (int n = 0; n < FW; n++) s[n] = reinterpret_cast<const int *>(rows)[16 * (ww * FW + n) + c];
+            for (int n = 0; n < FW; n++) s[n] = rows[16 * (ww * FW + n)];
 #pragma unroll
-                for (int m = 0; m < FX; m++) s[FW + m] = reinterpret_cast<const int *>(rows)[16 * (TW + wx * FX + m) + c];
-            } else {
-                read_scales(rows + 64 * ww * FW, rows + 64 * (TW + wx * FX), c, s);
-            }
+            for (int m = 0; m < FX; m++) s[FW + m] = rows[16 * (TW + wx * FX + m)];
         }
         i8 a[FW], b[FX];
-        if constexpr (STAGES == 1) {
-            a[0] = load_tile(stage + ww * FW * kQTileBytes, lane);
+        a[0] = load_tile(stage + ww * FW * kQTileBytes, lane);
 #pragma unroll
-            for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
+        for (int m = 0; m < FX; m++) b[m] = load_tile(stage + (TW + wx * FX + m) * kQTileBytes, lane);
 #pragma unroll
-            for (int n = 1; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
-        } else {
-            read_tiles(stage + ww * FW * kQTileBytes, stage + (TW + wx * FX) * kQTileBytes, lane, a, b);
-        }
+        for (int n = 1; n < FW; n++) a[n] = load_tile(stage + (ww * FW + n) * kQTileBytes, lane);
         if constexpr (STAGES == 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                   // ... and read by all
         }
         __builtin_amdgcn_sched_barrier(0);
         // on its way while the products run (behind the last block: that one again, without a branch around the copies)
-        fetch(min(kb + kAhead, blocks - 1), (kb + kAhead) % STAGES);
+        fetch(min(kb + 1, blocks - 1), (kb + 1) % STAGES);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < FW; n++)
@@ -554,8 +451,7 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
             for (int m = 0; m < FX; m++) acc[n][m] = scaled_product<EXACT, J>(a[n], b[m], acc[n][m], s[n], s[FW + m]);
     };
     fetch_scales(0);
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) fetch(min(k, blocks - 1), k);
+    fetch(0, 0);
     for (int kb = 0; kb < blocks; kb += 4) {
         step(kb, std::integral_constant<int, 0>());
         if (kb + 4 < blocks) fetch_scales(kb / 4 + 1);
@@ -764,13 +660,19 @@ hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream)
 
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
-    if (tiles(p, 128, 64) < 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
-    if (p.y_type == LCRC_T_F32) {
-        if (tiles(p, 128, 128) >= 256) tile_launch<true, 8, 2, 1, 4, 2>(p, stream);
-        else tile_launch<true, 8, 1, 1, 4, 3>(p, stream);
-    } else if (tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
-    else if (tiles(p, 128, 128) >= 256) tile_launch<false, 8, 2, 1, 4, 2>(p, stream);
-    else tile_launch<false, 8, 1, 1, 4, 3>(p, stream);
+    // Which tiles (measured, us): large ones read least per product, but need two workgroups for every CU:
+    //   4096 x 8192 x 2048 bf16   256 x 128 (256 tiles) 86, 128 x 128 (512) 73, 128 x 64 100
+    //   777 x 1999 x 2309 f16     128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
+    // In short sums nothing is read often enough to count, and small tiles fill the card better:
+    //   8192 x 372 x 1500 in 8 bits  128 x 128 22.9, 128 x 64 19.4
+    const bool exact = p.y_type == LCRC_T_F32, longer = p.n_in > 512;
+    if (tiles(p, 128, 64) <= 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
+    if (exact) {
+        if (longer && tiles(p, 128, 128) >= 512) tile_launch<true, 8, 2, 1, 4>(p, stream);
+        else tile_launch<true, 8, 1, 1, 4, 2>(p, stream);
+    } else if (longer && tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
+    else if (longer && tiles(p, 128, 128) >= 512) tile_launch<false, 8, 2, 1, 4>(p, stream);
+    else tile_launch<false, 8, 1, 1, 4, 2>(p, stream);
     return hipGetLastError();
 }
 
