@@ -269,6 +269,19 @@ typedef struct lcrc_fp8_linear_args {
 size_t lcrc_fp8_linear_workspace(int rows, int n_in, int x_type);
 int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *args, void *hip_stream);
 
+/* The two operators on a context's own nets.
+ * lcrc_posteriors_scored: lcrc_posteriors_batch with the scores of the posteriors beside them, computed where they are
+ * (lcrc_score, LCRC_SCORE_PROBS): host pointers, rows as in `post`; labels[rows][n_labels], outputs as lcrc_score names them,
+ * any of them and `post` NULL when not wanted.  Of plain posteriors: refused while lcrc_output_configure changes them.  The
+ * decoder on the device does not run in this call.
+ * lcrc_set_merger_fp8: the merger of the systems that lcrc_create_system runs from memory (1BT_DCT, 1BT, 3BT and LCRC at any
+ * other geometry than the shipped ones) with 8-bit operands: normalised inputs, weights and hidden activations in e4m3 with
+ * a scale per 128, sums, biases, sigmoid, softmax and output transform as ever.  Opt-in: the operands keep 4 significant
+ * bits, so posteriors are a few 1e-2 from those of the 32-bit nets.  The shipped LCRC shapes: LCRC_E_UNSUPPORTED. */
+int lcrc_posteriors_scored(lcrc_ctx *ctx, const float *mel, const int *off, int n_utts, float *post, const int *labels, int n_labels,
+                           int k, float *logp, float *entropy, int *top_index, float *top_logp);
+int lcrc_set_merger_fp8(lcrc_ctx *ctx, int enabled);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ SYMBOLS = [
     "lcrc_reset", "lcrc_push", "lcrc_delay",
     "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_kernel_name",
     "lcrc_score_workspace", "lcrc_score", "lcrc_fp8_bytes", "lcrc_fp8_pack", "lcrc_fp8_unpack", "lcrc_fp8_linear_workspace", "lcrc_fp8_linear",
+    "lcrc_posteriors_scored", "lcrc_set_merger_fp8",
 ]
 
 LCRC_OK, LCRC_E_ARG, LCRC_E_IO, LCRC_E_MODEL, LCRC_E_DEVICE, LCRC_E_NOMEM, LCRC_E_UNSUPPORTED = \
@@ -189,6 +190,8 @@ def load():
     L.lcrc_fp8_unpack.argtypes = [C.c_int, vp, C.c_int, C.c_int, vp, C.c_int, C.c_longlong, vp]
     L.lcrc_fp8_linear_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
     L.lcrc_fp8_linear.argtypes = [C.c_int, C.POINTER(Fp8LinearArgs), vp]
+    L.lcrc_posteriors_scored.argtypes = [vp, _f32p, vp, C.c_int, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp]
+    L.lcrc_set_merger_fp8.argtypes = [vp, C.c_int]
     for name in ("lcrc_score_workspace", "lcrc_fp8_bytes", "lcrc_fp8_linear_workspace"):
         getattr(L, name).restype = C.c_size_t
     _lib = L
@@ -538,6 +541,27 @@ class Lcrc:
     def set_arithmetic(self, arithmetic):
         """ARITH_F32 (default) or ARITH_SPLIT_F16 (f32 products as three exact f16 MFMA products; shipped LCRC shapes)"""
         self._check(self.L.lcrc_set_arithmetic(self.h, arithmetic))
+
+    def set_merger_fp8(self, enabled):
+        """the merger with 8-bit operands (systems other than the shipped LCRC shapes; lcrc_set_merger_fp8)"""
+        self._check(self.L.lcrc_set_merger_fp8(self.h, int(enabled)))
+
+    def posteriors_scored(self, mel, off, labels=None, k=0):
+        """posteriors_batch with their scores: dict of post, entropy and, as asked for, logp [rows][n_labels] of the labels
+        (negative: none), top_index and top_logp [rows][k] (lcrc_posteriors_scored)"""
+        mel = np.ascontiguousarray(mel, dtype=np.float32).reshape(-1, self.nbanks)
+        off = np.ascontiguousarray(off, dtype=np.int32)
+        rows = mel.shape[0]
+        m = 0
+        if labels is not None:
+            labels = np.ascontiguousarray(labels, dtype=np.int32).reshape(rows, -1)
+            m = labels.shape[1]
+        out = dict(post=np.zeros((rows, self.n_out), np.float32), entropy=np.zeros(rows, np.float32), logp=np.zeros((rows, m), np.float32),
+                   top_index=np.zeros((rows, max(k, 0)), np.int32), top_logp=np.zeros((rows, max(k, 0)), np.float32))
+        p = {n: a.ctypes.data for n, a in out.items()}
+        self._check(self.L.lcrc_posteriors_scored(self.h, mel, off.ctypes.data, len(off) - 1, p["post"], labels.ctypes.data if m else None, m, k,
+                                                  p["logp"], p["entropy"], p["top_index"], p["top_logp"]))
+        return out
 
     def set_wait_mode(self, poll_interval_us):
         self._check(self.L.lcrc_set_wait_mode(self.h, int(poll_interval_us)))

@@ -119,8 +119,9 @@ struct RawBlock {
     }
 };
 
-// One wave per tile of 16 rows x 128 columns.
-template <typename X>
+// One wave per tile of 16 rows x 128 columns.  NORM: the values are normalised first, (v - mean[column]) * dev[column]
+// (Normalize, nn.cpp:702-716).
+template <typename X, bool NORM = false>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
 {
     const Q8Shape s(p.rows, p.cols);
@@ -151,6 +152,13 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
         RawBlock<X> raw;
         raw.load(src, kb, p.cols, g);
         raw.values(v, live, kb, p.cols, g);
+        if constexpr (NORM) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const long long k = kb * 128 + column_of(g, j);
+                if (live && k < p.cols) v[j] = (v[j] - p.mean[k]) * p.dev[k];
+            }
+        }
         q = quantise(v, &e);
     }
     store_tile(p.dst + tile * kQTileBytes, lane, q);
@@ -637,6 +645,10 @@ hipError_t fp8_pack_launch(const Fp8PackParams &p, hipStream_t stream)
 {
     const Q8Shape s(p.rows, p.cols);
     const unsigned blocks = (unsigned)((s.rt * s.kb + 3) / 4);
+    if (p.mean) {
+        fp8_pack_kernel<float, true><<<blocks, 256, 0, stream>>>(p);
+        return hipGetLastError();
+    }
     switch (p.type) {
     case LCRC_T_F32: fp8_pack_kernel<float><<<blocks, 256, 0, stream>>>(p); break;
     case LCRC_T_F16: fp8_pack_kernel<_Float16><<<blocks, 256, 0, stream>>>(p); break;

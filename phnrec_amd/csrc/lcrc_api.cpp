@@ -526,8 +526,9 @@ int launch_traps(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, 
 {
     if (n_rows <= 0) return LCRC_OK;
     const size_t Km = c->nets[2].n_inp;
-    const bool fused_dct = c->system == SYS_1BT_DCT && !c->traps_unfused;
-    const bool fused_bt = c->system != SYS_1BT_DCT && !c->traps_unfused && !c->bt_unfused;
+    const bool unfused = c->traps_unfused || c->fp8_merger;        // (the 8-bit merger reads its inputs from memory)
+    const bool fused_dct = c->system == SYS_1BT_DCT && !unfused;
+    const bool fused_bt = c->system != SYS_1BT_DCT && !unfused && !c->bt_unfused;
     if (!fused_dct && !fused_bt && (size_t)n_rows > c->cap_feat_rows) {
         const size_t cap = (size_t)n_rows + n_rows / 4 + 64;
         if (c->d_feat) (void)hipFree(c->d_feat);
@@ -607,7 +608,10 @@ int launch_traps(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, 
     m.out = d_post; m.out_ld = c->nets[2].n_out;
     m.neg_log = 0;
     fill_output_transform(c, m.out_func, m.out_c, m.out_l, &m.out_be);
-    HIP_TRY(c, mlp_launch(m, s, &c->mlp_variant));
+    if (c->fp8_merger) {
+        const int rc = merger_fp8(c, merger_in, n_rows, m, s);
+        if (rc) return rc;
+    } else HIP_TRY(c, mlp_launch(m, s, &c->mlp_variant));
     if (c->timing) { HIP_TRY(c, hipEventRecord(c->ev1, s)); c->timed = true; }
     return LCRC_OK;
 }
@@ -787,8 +791,8 @@ int two_part_output(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utt
     return LCRC_OK;
 }
 
-int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, float *post,
-             float *const *probes, bool decode = true)
+int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, float *post, float *const *probes, bool decode,
+             const HostScores *scores)
 {
     const size_t nb = c->nbanks, O = c->nets[2].n_out;
     int rc = ensure_staging(c, n, n_utts);
@@ -817,14 +821,14 @@ int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, f
             for (int i = 0; i < 5; i++) dbg[i] = probes[i] ? c->d_dbg[i] : nullptr;
         }
     }
-    if (!any && !(decode && c->dec_P > 0)) {
+    if (!any && !scores && !(decode && c->dec_P > 0)) {
         bool done = false;
         rc = two_part_output(c, c->d_mel, d_off, off ? n_utts : 1, n, post, &done);
         if (rc || done) return rc;
     }
     float *out_dev = c->d_post;
     bool direct = false;
-    rc = output_target(c, !(decode && c->dec_P > 0) || c->readback, post == nullptr, &out_dev, &direct);
+    if (!scores) rc = output_target(c, !(decode && c->dec_P > 0) || c->readback, post == nullptr, &out_dev, &direct);
     if (rc) return rc;
     rc = launch(c, c->d_mel, d_off, off ? n_utts : 1, n, out_dev, c->stream, any ? dbg : nullptr);
     if (rc) return rc;
@@ -837,7 +841,11 @@ int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, f
         rc = decode_after(c, c->d_off, c->h_off, off ? n_utts : 1, n, c->d_post, c->stream);
         if (rc) return rc;
     }
-    const bool copy_post = c->readback || !decoding;
+    if (scores) {
+        rc = scores_after(c, *scores, n, c->d_post);
+        if (rc) return rc;
+    }
+    const bool copy_post = scores ? post != nullptr : c->readback || !decoding;
     if (copy_post && direct) {
         HIP_TRY(c, wait_stream(c));
         if (post) memcpy(post, c->h_post, (size_t)n * O * sizeof(float));
@@ -848,6 +856,7 @@ int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, f
     } else {
         HIP_TRY(c, wait_stream(c));
     }
+    if (scores) fetch_scores(c, *scores, n);
     if (any)
         for (int i = 0; i < 5; i++)
             if (probes[i]) HIP_TRY(c, hipMemcpy(probes[i], c->d_dbg[i], (size_t)n * widths[i] * sizeof(float), hipMemcpyDeviceToHost));
@@ -1279,6 +1288,9 @@ void lcrc_destroy(lcrc_ctx *c)
     if (c->h_count) (void)pinned_free(c->h_count);
     if (c->d_feat) (void)hipFree(c->d_feat);
     if (c->d_minp) (void)hipFree(c->d_minp);
+    if (c->d_fp8) (void)hipFree(c->d_fp8);
+    if (c->d_scores) (void)hipFree(c->d_scores);
+    if (c->h_scores) (void)pinned_free(c->h_scores);
     if (c->d_hamming) (void)hipFree(c->d_hamming);
     if (c->d_coeffs) (void)hipFree(c->d_coeffs);
     if (c->d_twiddle) (void)hipFree(c->d_twiddle);

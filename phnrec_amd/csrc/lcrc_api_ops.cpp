@@ -60,7 +60,178 @@ int check_held(const char *call, const void *p, int rows, int cols)
 
 }  // namespace
 
+namespace lcrc_impl {
+
+// ---- the merger of an unfused system with 8-bit operands (lcrc_set_merger_fp8) ----
+// inputs -> normalised, in 8 bits -> hidden layer (FEXP sigmoid), in 8 bits -> outputs in f32 -> softmax and output transform
+int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, hipStream_t s)
+{
+    const NetDev &net = c->nets[2];
+    const size_t x_bytes = (size_t)Q8Shape(n_rows, net.n_inp).bytes(), h_bytes = (size_t)Q8Shape(n_rows, net.n_hid).bytes();
+    const size_t need = x_bytes + h_bytes + (size_t)n_rows * net.n_out * sizeof(float);
+    if (need > c->cap_fp8) {
+        if (c->d_fp8) (void)hipFree(c->d_fp8);              // (waits for launches that still use it)
+        c->d_fp8 = nullptr;
+        c->cap_fp8 = 0;
+        if (dev_alloc((void **)&c->d_fp8, need + need / 4) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail(c, LCRC_E_NOMEM, "cannot allocate the 8-bit merger's operands for " + std::to_string(n_rows) + " frames");
+        }
+        c->cap_fp8 = need + need / 4;
+    }
+    unsigned char *x = c->d_fp8, *h = x + x_bytes;
+    float *y = reinterpret_cast<float *>(h + h_bytes);
+    Fp8PackParams pack = {d_in, nullptr, LCRC_T_F32, n_rows, net.n_inp, net.n_inp, x, net.mean, net.dev};
+    HIP_TRY(c, fp8_pack_launch(pack, s));
+    HIP_TRY(c, fp8_product_launch({x, c->fp8_w1, net.b1, n_rows, net.n_inp, net.n_hid, LCRC_ACT_FSIGMOID, LCRC_T_E4M3, h, 0}, s));
+    HIP_TRY(c, fp8_product_launch({h, c->fp8_w2, net.b2, n_rows, net.n_hid, net.n_out, LCRC_ACT_NONE, LCRC_T_F32, y, net.n_out}, s));
+    SoftmaxRowsParams o;
+    memset(&o, 0, sizeof o);
+    o.in = y; o.out = m.out; o.out_ld = m.out_ld; o.n_rows = n_rows; o.n = net.n_out;
+    memcpy(o.out_func, m.out_func, sizeof o.out_func);
+    memcpy(o.out_c, m.out_c, sizeof o.out_c);
+    memcpy(o.out_l, m.out_l, sizeof o.out_l);
+    o.out_be = m.out_be;
+    HIP_TRY(c, softmax_rows_launch(o, s));
+    return LCRC_OK;
+}
+
+// ---- scores behind the posteriors (lcrc_posteriors_scored) ----
+namespace {
+// one block: [labels][ln p of them][entropy][best classes][their ln p] (labels and scores: also in pinned memory), scratch
+struct ScoreLayout {
+    size_t labels, logp, entropy, index, top, host_end, end;
+    ScoreLayout(const lcrc_ctx *c, const HostScores &w, size_t n)
+    {
+        size_t at = 0;
+        const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+        labels = take(n * w.n_labels * sizeof(int));
+        logp = take(n * w.n_labels * sizeof(float));
+        entropy = take(n * sizeof(float));
+        index = take(n * w.k * sizeof(int));
+        top = take(n * w.k * sizeof(float));
+        host_end = at;
+        end = at + score_workspace_bytes((int)n, c->nets[2].n_out, w.k);
+    }
+};
+}  // namespace
+
+int scores_after(lcrc_ctx *c, const HostScores &w, int n_rows, const float *d_post)
+{
+    const ScoreLayout l(c, w, n_rows);
+    if (l.end > c->cap_scores) {
+        if (c->d_scores) (void)hipFree(c->d_scores);
+        if (c->h_scores) (void)pinned_free(c->h_scores);
+        c->d_scores = c->h_scores = nullptr;
+        c->cap_scores = 0;
+        const size_t cap = l.end + l.end / 4;
+        if (dev_alloc((void **)&c->d_scores, cap) != hipSuccess || pinned_alloc((void **)&c->h_scores, cap) != hipSuccess) {
+            if (c->d_scores) (void)hipFree(c->d_scores);
+            c->d_scores = c->h_scores = nullptr;
+            (void)hipGetLastError();
+            return fail(c, LCRC_E_NOMEM, "cannot allocate the scores of " + std::to_string(n_rows) + " frames");
+        }
+        c->cap_scores = cap;
+    }
+    char *d = c->d_scores, *h = c->h_scores;
+    if (w.n_labels > 0) {
+        const size_t bytes = (size_t)n_rows * w.n_labels * sizeof(int);
+        memcpy(h + l.labels, w.labels, bytes);
+        HIP_TRY(c, hipMemcpyAsync(d + l.labels, h + l.labels, bytes, hipMemcpyHostToDevice, c->stream));
+    }
+    lcrc_score_args a;
+    memset(&a, 0, sizeof a);
+    a.x = d_post; a.type = LCRC_T_F32; a.form = LCRC_SCORE_PROBS;
+    a.rows = n_rows; a.cols = c->nets[2].n_out; a.ld = a.cols;
+    a.labels = (const int *)(d + l.labels); a.n_labels = w.n_labels; a.k = w.k;
+    a.logp = w.n_labels > 0 ? (float *)(d + l.logp) : nullptr;
+    a.entropy = (float *)(d + l.entropy);
+    a.top_index = w.k > 0 ? (int *)(d + l.index) : nullptr;
+    a.top_logp = w.k > 0 ? (float *)(d + l.top) : nullptr;
+    a.workspace = d + l.host_end; a.workspace_bytes = l.end - l.host_end;
+    HIP_TRY(c, score_launch(a, c->stream));
+    HIP_TRY(c, hipMemcpyAsync(h + l.logp, d + l.logp, l.host_end - l.logp, hipMemcpyDeviceToHost, c->stream));
+    return LCRC_OK;
+}
+
+void fetch_scores(lcrc_ctx *c, const HostScores &w, int n_rows)
+{
+    const ScoreLayout l(c, w, n_rows);
+    const size_t n = n_rows;
+    const char *h = c->h_scores;
+    if (w.logp) memcpy(w.logp, h + l.logp, n * w.n_labels * sizeof(float));
+    if (w.entropy) memcpy(w.entropy, h + l.entropy, n * sizeof(float));
+    if (w.top_index) memcpy(w.top_index, h + l.index, n * w.k * sizeof(int));
+    if (w.top_logp) memcpy(w.top_logp, h + l.top, n * w.k * sizeof(float));
+}
+
+}  // namespace lcrc_impl
+
 extern "C" {
+
+int lcrc_set_merger_fp8(lcrc_ctx *c, int enabled)
+{
+    if (!c) return LCRC_E_ARG;
+    if (!enabled) { c->fp8_merger = false; return LCRC_OK; }
+    if (c->system == SYS_LCRC)
+        return fail(c, LCRC_E_UNSUPPORTED, "lcrc_set_merger_fp8: the fused LCRC kernels hold their operands in f32 or split f16");
+    HIP_TRY(c, hipSetDevice(c->device));
+    if (!c->fp8_w1) {
+        const HostNet &net = c->model->host[2];
+        for (const std::vector<float> *w : {&net.w1, &net.w2})
+            for (float v : *w)
+                if (!std::isfinite(v)) return fail(c, LCRC_E_UNSUPPORTED, "lcrc_set_merger_fp8: non-finite weights have no 8-bit form");
+        const size_t bytes1 = lcrc_fp8_bytes(net.n_hid, net.n_inp), bytes2 = lcrc_fp8_bytes(net.n_out, net.n_hid);
+        void *w1 = nullptr, *w2 = nullptr, *rows = nullptr;
+        const auto pack = [&](const std::vector<float> &w, int n_out, int n_in, void *dst) {
+            if (const hipError_t e = hipMemcpy(rows, w.data(), w.size() * sizeof(float), hipMemcpyHostToDevice); e != hipSuccess) return e;
+            if (const hipError_t e = fp8_pack_launch({rows, nullptr, LCRC_T_F32, n_out, n_in, n_in, (unsigned char *)dst, nullptr, nullptr}, c->stream);
+                e != hipSuccess) return e;
+            return hipStreamSynchronize(c->stream);
+        };
+        hipError_t e = dev_alloc(&w1, bytes1);
+        if (e == hipSuccess) e = dev_alloc(&w2, bytes2);
+        if (e == hipSuccess) e = dev_alloc(&rows, std::max(net.w1.size(), net.w2.size()) * sizeof(float));
+        const bool room = e == hipSuccess;
+        if (e == hipSuccess) e = pack(net.w1, net.n_hid, net.n_inp, w1);
+        if (e == hipSuccess) e = pack(net.w2, net.n_out, net.n_hid, w2);
+        if (rows) (void)hipFree(rows);
+        if (e != hipSuccess) {
+            if (w1) (void)hipFree(w1);
+            if (w2) (void)hipFree(w2);
+            (void)hipGetLastError();
+            return fail(c, room ? LCRC_E_DEVICE : LCRC_E_NOMEM, std::string("lcrc_set_merger_fp8: ") + hipGetErrorString(e));
+        }
+        c->allocs.push_back(w1);
+        c->allocs.push_back(w2);
+        c->fp8_w1 = (unsigned char *)w1;
+        c->fp8_w2 = (unsigned char *)w2;
+    }
+    c->fp8_merger = true;
+    return LCRC_OK;
+}
+
+int lcrc_posteriors_scored(lcrc_ctx *c, const float *mel, const int *off, int n_utts, float *post, const int *labels, int n_labels,
+                           int k, float *logp, float *entropy, int *top_index, float *top_logp)
+{
+    const auto bad_arg = [&](const char *what) { return fail(c, LCRC_E_ARG, std::string("lcrc_posteriors_scored: ") + what); };
+    if (!c) return LCRC_E_ARG;
+    if (n_utts < 0 || (n_utts > 0 && !off)) return bad_arg("bad argument");
+    if (n_labels < 0 || n_labels > kScoreMaxLabels) return bad_arg("n_labels: 0 .. 64");
+    if (k < 0 || k > kScoreMaxTop || k > c->nets[2].n_out) return bad_arg("k: 0 .. 64, at most the model's outputs");
+    if (n_utts == 0) return LCRC_OK;
+    if (off[0] != 0) return bad_arg("off[0] must be 0");
+    for (int u = 0; u < n_utts; u++)
+        if (off[u + 1] < off[u]) return bad_arg("offsets must be non-decreasing");
+    const int n = off[n_utts];
+    if (n == 0) return LCRC_OK;
+    if (!mel || (n_labels > 0 && !labels)) return bad_arg("NULL buffer");
+    if (c->soft[0].func != LCRC_SOFT_NONE || c->soft[1].func != LCRC_SOFT_NONE || c->out_be)
+        return bad_arg("scores are taken of plain posteriors (lcrc_output_configure without stages, in host byte order)");
+    HIP_TRY(c, hipSetDevice(c->device));
+    const HostScores want = {labels, n_labels, k, logp, entropy, top_index, top_logp};
+    return run_host(c, mel, off, n_utts, n, post, nullptr, false, &want);
+}
 
 size_t lcrc_score_workspace(int rows, int cols, int k)
 {
@@ -108,7 +279,7 @@ int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, 
     if (const int rc = check_held(call, dst, rows, cols)) return rc;
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
-    const Fp8PackParams p = {src, scales, type, rows, cols, ld, static_cast<unsigned char *>(dst)};
+    const Fp8PackParams p = {src, scales, type, rows, cols, ld, static_cast<unsigned char *>(dst), nullptr, nullptr};
     return launched(call, fp8_pack_launch(p, static_cast<hipStream_t>(hip_stream)));
 }
 
@@ -159,7 +330,7 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     Fp8ProductParams p = {x, static_cast<const unsigned char *>(a->w), a->bias, a->rows, a->n_in, a->n_out, a->act, a->y_type, a->y, a->ldy};
     if (a->x_type != LCRC_T_E4M3) {
         if (a->rows <= kQRows && a->n_out <= kQFewOut) return launched(call, fp8_few_rows_launch(p, a->x, a->x_type, a->ldx, s));
-        const Fp8PackParams pack = {a->x, nullptr, a->x_type, a->rows, a->n_in, a->ldx, static_cast<unsigned char *>(a->workspace)};
+        const Fp8PackParams pack = {a->x, nullptr, a->x_type, a->rows, a->n_in, a->ldx, static_cast<unsigned char *>(a->workspace), nullptr, nullptr};
         if (const int rc = launched(call, fp8_pack_launch(pack, s))) return rc;
         p.x = pack.dst;
     }

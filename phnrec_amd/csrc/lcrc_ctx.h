@@ -135,6 +135,13 @@ struct lcrc_ctx {
     int out_be = 0;
     int tile_frames = 0;
     int arith = 0;              // LCRC_ARITH_*
+    // lcrc_set_merger_fp8: the merger's weights in the 8-bit form (among allocs), its operands of one launch
+    bool fp8_merger = false;
+    unsigned char *fp8_w1 = nullptr, *fp8_w2 = nullptr, *d_fp8 = nullptr;
+    size_t cap_fp8 = 0;
+    // lcrc_posteriors_scored: labels, scores and scratch on the device, labels and scores in pinned host memory
+    char *d_scores = nullptr, *h_scores = nullptr;
+    size_t cap_scores = 0;
     // decoder on the device ("next" row f3): configuration, label buffers (device + pinned host)
     int dec_P = 0, dec_S = 0, dec_prune = 0;
     float dec_wpen = 0.f;
@@ -193,6 +200,17 @@ constexpr unsigned kPinned = hipHostMallocPortable;
 constexpr unsigned kPinnedMapped = hipHostMallocPortable | hipHostMallocMapped | hipHostMallocCoherent;
 constexpr int kCopyPieces = 4;           // <= lcrc_ctx::ev_piece
 
+// lcrc_posteriors_scored: what the caller gives and wants (host pointers)
+struct HostScores {
+    const int *labels;
+    int n_labels, k;
+    float *logp, *entropy;
+    int *top_index;
+    float *top_logp;
+};
+// ---- lcrc_api_ops.cpp: behind the posteriors of a host call on c->stream, and after the wait for it
+int scores_after(lcrc_ctx *c, const HostScores &w, int n_rows, const float *d_post);
+void fetch_scores(lcrc_ctx *c, const HostScores &w, int n_rows);
 // ---- lcrc_api.cpp ----
 hipError_t dev_alloc(void **p, size_t bytes);
 hipError_t pinned_alloc(void **p, size_t bytes, bool device_reads = false);
@@ -206,6 +224,8 @@ int output_target(lcrc_ctx *c, bool copy_post, bool in_place, float **out, bool 
 void ensure_split_scratch(lcrc_ctx *c);
 int launch(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, int n_rows, float *d_post,
            hipStream_t s, float *const *dbg, int row_first = 0, int row_count = -1, bool timed = true);
+int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, float *post, float *const *probes, bool decode = true,
+             const HostScores *scores = nullptr);
 int two_part_output(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, int n, float *post, bool *done);
 
 // ---- lcrc_api_decoder.cpp ----
@@ -223,6 +243,9 @@ struct OverlapScope {
 };
 int decode_after(lcrc_ctx *c, const int *d_off, const int *h_first, int n_utts, int n_rows, const float *d_post,
                  hipStream_t s, bool staged = false);
+
+// ---- lcrc_api_ops.cpp ----
+int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, hipStream_t s);
 
 }  // namespace lcrc_impl
 

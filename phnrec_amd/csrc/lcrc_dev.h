@@ -173,6 +173,19 @@ hipError_t mlp_launch(const MlpParams &p, hipStream_t stream, const char **varia
 hipError_t traps_1bt_launch(const MlpParams &p, hipStream_t stream, const char **variant = nullptr);
 bool mlp_supports(const NetDev &net);
 
+// rows of a net's outputs before the softmax -> posteriors: softmax (nn.cpp:822-855), softening, byte order
+struct SoftmaxRowsParams {
+    const float *in;     // [n_rows][n], tight
+    float *out;          // row r at out + r * out_ld
+    long out_ld;
+    int n_rows, n;       // n <= 1024
+    int out_func[2];
+    float out_c[2][4];
+    float out_l[2][2];
+    int out_be;
+};
+hipError_t softmax_rows_launch(const SoftmaxRowsParams &p, hipStream_t stream);
+
 // ---- phoneme-loop Viterbi decoder (phndec_kernels.hip; "next" row f3, optional) ---------------------
 struct PhnDecParams {
     const float *logpost;   // [rows][cols] softened (log) posteriors, resident in HBM

@@ -45,6 +45,7 @@ struct Fp8PackParams {
     int type, rows, cols;
     long long ld;
     unsigned char *dst;
+    const float *mean, *dev;       // type f32: [cols], or NULL: the values are normalised before they are rounded
 };
 struct Fp8UnpackParams {
     const unsigned char *src;
