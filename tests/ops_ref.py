@@ -1,6 +1,26 @@
 """Plain 64-bit implementations of the operators on matrices in device memory (include/lcrc_pipeline.h), for their tests."""
 import numpy as np
 
+
+class _Torch:
+    """torch, imported when it is first used: a test process that collects the tests without running them stays small (other
+    tests measure the memory of the processes they start, which begins with their parent's)"""
+
+    def __getattr__(self, name):
+        import torch
+        return getattr(torch, name)
+
+
+torch = _Torch()
+
+
+class _Types:
+    def __getitem__(self, name):
+        return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+DT = _Types()
+
 EPS = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}       # a rounding is off by at most this, relative
 
 

@@ -6,9 +6,7 @@ from tests import ops_ref as ref
 
 pytestmark = pytest.mark.gpu
 
-torch = pytest.importorskip("torch")
-
-DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+torch, DT = ref.torch, ref.DT
 
 
 @pytest.fixture(scope="module")

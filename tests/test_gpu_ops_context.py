@@ -7,11 +7,11 @@ import pytest
 
 from phnrec_amd import modelgen
 from tests import ops_ref as ref
-from tests.test_gpu_ops import DT, Linear, Scored, _activations, _close, _pack, _stream, _weights
+from tests.test_gpu_ops import Linear, Scored, _activations, _close, _stream, _weights
 
 pytestmark = pytest.mark.gpu
 
-torch = pytest.importorskip("torch")
+torch = ref.torch
 
 EPS = ref.EPS["f32"]
 
