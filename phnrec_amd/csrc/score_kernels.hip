@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
     }
 }
 
-// ---- longer rows: the best classes by a threshold ----
+// ---- longer rows, longer lists: the best classes by a threshold ----
 // A key orders values, then columns (or chunks, or positions): 32 bits that rise with the value, -0 and +0 alike, and the
 // complement of the column below them; 0 is below every key of a value.
 __device__ __forceinline__ unsigned ordered(float x)
@@ -277,7 +277,8 @@ __device__ __forceinline__ u64 bar_of(const u64 (&key)[G], int k)
 constexpr int kCandidates = 512;       // candidates a team holds (more: the slow way)
 
 // A team of threads that works on one row: T threads, one wave or a whole workgroup.
-template <int T>
+// TOGETHER: a wave that looks through its values in step, and needs no counter in memory.
+template <int T, bool TOGETHER = false>
 struct Team {
     static constexpr int kWaves = T / 64;
     struct Shared {
@@ -352,17 +353,20 @@ struct Team {
     }
     // The k best of the team's values, best first: out(rank, key), by the thread that finds it.
     //   first          the bests (value, chunk) of this thread's shares, as keys, 0 where it has none
-    //   scan(bar, f)   f(value, chunk, column) for what this thread holds, at least for the values whose keys reach the bar
+    //   scan(bar, f)   f(live, value, chunk, column) for what this thread holds, at least for the values whose keys reach the
+    //                  bar; by a whole wave together where the team is one
+    //   again(f)       the same for all that it holds, any number of times
     // The threads' shares are put into 64 G groups.  The k-th best of the groups' bests is reached by at least k values, so
     // the k best are among the values that reach it, and only threads with such a group look at their values again.  With
     // 256 groups some 74 of random values remain for k = 64, 17 for k = 16 (from 64 groups 300 and 18).  They are ranked by
     // counting.  Rows made so that more remain than fit are done one rank after another.
-    template <int N, typename Scan, typename Out>
-    __device__ __forceinline__ void top(int k, const u64 (&first)[N], const Scan &scan, const Out &out)
+    template <int N, typename Scan, typename Again, typename Out>
+    __device__ __forceinline__ void top(int k, const u64 (&first)[N], const Scan &scan, const Again &again, const Out &out)
     {
+        static_assert(N == 1 || T == 64, "a workgroup's threads are groups of one share each");
         constexpr int G = T > 64 ? 4 : N;
         u64 group[G];
-        if (t == 0) sh.count = 0;
+        if (!TOGETHER && t == 0) sh.count = 0;
         if constexpr (T > 64) {
             sh.best[t] = first[0];
             sync();
@@ -377,18 +381,34 @@ struct Team {
             sync();
         }
         const u64 bar = bar_of(group, k);
-        bool look = false;
+        const float least = key_value(bar);
+        const auto reaches = [&](float v, int chunk) {          // (a bar between two values can lie at a NaN: no help then)
+            return !(v < least) && make_key(v, chunk) >= bar;
+        };
+        int n = 0;
+        if constexpr (!TOGETHER) {
+            bool look = false;
 #pragma unroll
-        for (int q = 0; q < N; q++) look = look || (first[q] >= bar && first[q] != 0);
-        if (look)
-            scan(bar, [&](float v, int chunk, int c) {
-                if (make_key(v, chunk) >= bar) {
-                    const int at = atomicAdd(&sh.count, 1);      // (any order: they are ranked by their keys)
-                    if (at < kCandidates) sh.cand[at] = make_key(v, c);
-                }
+            for (int q = 0; q < N; q++) look = look || (first[q] >= bar && first[q] != 0);
+            if (look)
+                scan(bar, [&](bool live, float v, int chunk, int c) {
+                    if (live && reaches(v, chunk)) {
+                        const int at = atomicAdd(&sh.count, 1);      // (any order: they are ranked by their keys)
+                        if (at < kCandidates) sh.cand[at] = make_key(v, c);
+                    }
+                });
+            sync();
+            n = sh.count;
+        } else {
+            scan(bar, [&](bool live, float v, int chunk, int c) {
+                const bool hit = live && reaches(v, chunk);
+                const u64 all = __ballot(hit);
+                const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(all >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)all, 0));
+                if (hit && at < kCandidates) sh.cand[at] = make_key(v, c);
+                n += __popcll(all);
             });
-        sync();
-        const int n = sh.count;
+            sync();
+        }
         if (n <= kCandidates) {
             for (int i = t; i < n; i += T) {
                 const u64 key = sh.cand[i];
@@ -401,9 +421,9 @@ struct Team {
             u64 last = ~0ull;
             for (int q = 0; q < k; q++) {
                 u64 best = 0;
-                scan(0, [&](float v, int, int c) {
+                again([&](bool live, float v, int, int c) {
                     const u64 key = make_key(v, c);
-                    if (key < last && key > best) best = key;
+                    if (live && key < last && key > best) best = key;
                 });
                 last = max_key(best);
                 if (t == 0) out(q, last);
@@ -425,60 +445,51 @@ __device__ __forceinline__ void put_top(const lcrc_score_args &a, size_t r, cons
     if (a.top_logp) a.top_logp[r * a.k + rank] = row.ln_p(key_value(key));
 }
 
-// ---- middle rows: a wave to a row, the row in its registers: J chunks of 16 bytes to a lane ----
-template <typename X, bool PROBS, int J>
+// ---- a wave to a row, the row in its registers: a chunk of 16 bytes to a lane (rows of up to 64 chunks, k beyond the lists') ----
+template <typename X, bool PROBS>
 __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_args a)
 {
     constexpr int W = 16 / sizeof(X);
-    __shared__ typename Team<64>::Shared shared[kThreads / 64];
-    Team<64> team(shared[threadIdx.x >> 6]);
-    const int lane = team.t, cols = a.cols;
+    __shared__ typename Team<64, true>::Shared shared[kThreads / 64];
+    Team<64, true> team(shared[threadIdx.x >> 6]);
+    const int lane = team.t, cols = a.cols, start = min(lane * W, cols - W), from = lane * W - start;
     const size_t stride = (size_t)gridDim.x * (kThreads / 64);
     for (size_t r = (size_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); r < (size_t)a.rows; r += stride) {
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
-        Chunk<X, W> raw[J];
-#pragma unroll
-        for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((64 * j + lane) * W, cols - W));
-        const auto each = [&](const auto &f) {
-#pragma unroll
-            for (int j = 0; j < J; j++) {
-                const int at = (64 * j + lane) * W, start = min(at, cols - W);
-#pragma unroll
-                for (int i = 0; i < W; i++)
-                    if (start + i >= at) f(raw[j][i], 64 * j + lane, start + i);
-            }
-        };
-        float m = kLowest, least = 0.0f;
+        const Chunk<X, W> raw = load_chunk<X, W>(x + start);
+        // a lane's label and its value: on their way while the row is worked on
+        const int label = a.logp && lane < a.n_labels ? a.labels[r * a.n_labels + lane] : -1;
+        const float labelled = to_f32(x[label < 0 || label >= cols ? 0 : label]);
+        float least = 0.0f;
         Stats s = {0.0f, 0.0f, 0.0f};
-        if constexpr (!PROBS) {
+        float most = raw[W - 1];                    // of the chunk, without what it shares with the one before
 #pragma unroll
-            for (int j = 0; j < J; j++)
+        for (int i = 0; i < W - 1; i++) most = i >= from ? fmaxf(most, raw[i]) : most;
+        if constexpr (!PROBS) s.m = reduce64(fmaxf(most, kLowest), Max());         // (lanes behind the end: the last chunk's)
 #pragma unroll
-                for (int i = 0; i < W; i++) m = fmaxf(m, raw[j][i]);       // (what is there twice does no harm)
-            s.m = m = reduce64(m, Max());
-        }
-        each([&](float v, int, int) {
+        for (int i = 0; i < W; i++) {
+            const float v = i >= from ? raw[i] : PROBS ? 0.0f : -INFINITY;
             if constexpr (PROBS) least = fminf(least, v);
-            add_value<PROBS>(v, m, s.S, s.T);
-        });
+            add_value<PROBS>(v, s.m, s.S, s.T);
+        }
         s.S = reduce64(s.S, Add());
         s.T = finish<PROBS>(reduce64(s.T, Add()));
         if constexpr (PROBS) least = reduce64(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
-        if (a.logp && lane < a.n_labels) a.logp[r * a.n_labels + lane] = label_score<X, PROBS>(a, x, row, r * a.n_labels + lane);
+        if (a.logp && lane < a.n_labels)
+            a.logp[r * a.n_labels + lane] = label < 0 ? 0.0f : label >= cols ? NAN : row.ln_p(labelled);
         if (!wants_top(a)) continue;
         if (row.bad) {
             if (lane < a.k) put_bad(a, r, lane);
             continue;
         }
-        constexpr int N = J > 1 ? 2 : 1;
-        u64 first[N] = {};
-        each([&](float v, int chunk, int) {
-            u64 &f = first[(chunk >> 6) % N];
-            f = max(f, make_key(v, chunk));
-        });
-        team.top(a.k, first, [&](u64, const auto &f) { each(f); }, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
+        const u64 first[1] = {from < W ? make_key(most, lane) : 0};
+        const auto scan = [&](const auto &f) {
+#pragma unroll
+            for (int i = 0; i < W; i++) f(i >= from, raw[i], lane, start + i);
+        };
+        team.top(a.k, first, [&](u64, const auto &f) { scan(f); }, scan, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
     }
 }
 
@@ -490,16 +501,18 @@ struct Part {
     u64 *keys;                  // [rows][parts][k], best first, 0 where a part has fewer
 };
 
+// (T = 64: a wave to a row, four of them in a workgroup)
 template <typename X, bool PROBS, int T>
-__global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, const Part p)
+__global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_args a, const Part p)
 {
     constexpr int W = 16 / sizeof(X), U = 4;
-    __shared__ typename Team<T>::Shared shared;
-    Team<T> team(shared);
+    constexpr int kTeams = kThreads / T;
+    __shared__ typename Team<T>::Shared shared[kTeams];
+    Team<T> team(shared[threadIdx.x / T]);
     const int t = team.t, cols = a.cols, n_chunks = (cols + W - 1) / W;
     const bool want_top = wants_top(a);
     const size_t jobs = (size_t)a.rows * p.parts;
-    for (size_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+    for (size_t job = (size_t)blockIdx.x * kTeams + threadIdx.x / T; job < jobs; job += (size_t)gridDim.x * kTeams) {
         const size_t r = job / p.parts;
         const int from = (int)(job - r * p.parts) * p.chunks, to = min(from + p.chunks, n_chunks);
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
@@ -577,8 +590,7 @@ __global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, 
         const auto look_at = [&](const Chunk<X, W> &raw, int c, const auto &f) {
             const long long at = c * (long long)W, start = min(at, (long long)cols - W);
 #pragma unroll
-            for (int i = 0; i < W; i++)
-                if (start + i >= at) f(raw[i], c, (int)start + i);
+            for (int i = 0; i < W; i++) f(start + i >= at, raw[i], c, (int)start + i);
         };
         const auto chunk = [&](int c) { return load_chunk<X, W>(x + min(c * (long long)W, (long long)cols - W)); };
         // bar: what f is looking for; mostly a thread has it in its best chunk alone
@@ -597,7 +609,7 @@ __global__ __launch_bounds__(T) void score_long_kernel(const lcrc_score_args a, 
             }
         };
         const u64 first[1] = {most_at < 0 ? 0 : make_key(most, most_at)};
-        team.top(a.k, first, scan, [&](int rank, u64 key) {
+        team.top(a.k, first, scan, [&](const auto &f) { scan(0, f); }, [&](int rank, u64 key) {
             if (p.parts == 1) put_top<PROBS>(a, r, row, rank, key);
             else list[rank] = key;
         });
@@ -634,34 +646,40 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
         const int n = p.parts * a.k;
         const auto key_at = [&](int i) { return keys[i % p.parts * a.k + i / p.parts]; };
         u64 first[1] = {};
+#pragma unroll 8
         for (int i = t; i < n; i += kThreads) first[0] = max(first[0], key_at(i));
         const auto scan = [&](u64, const auto &f) {
-            for (int i = t; i < n; i += kThreads)
-                if (const u64 key = key_at(i)) f(key_value(key), key_column(key), key_column(key));
+#pragma unroll 8
+            for (int i = t; i < n; i += kThreads) {
+                const u64 key = key_at(i);
+                f(key != 0, key_value(key), key_column(key), key_column(key));
+            }
         };
-        team.top(a.k, first, scan, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
+        team.top(a.k, first, scan, [&](const auto &f) { scan(0, f); }, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
     }
 }
 
 // ---- which kernel, on what grid ----
-constexpr int kLongThreads = 512;
 constexpr int kMaxBlocks = 1 << 22;      // beyond it the workgroups take several rows each
 
 Part parts_of(int rows, int cols, int type)
 {
     const int w = type == LCRC_T_F32 ? 4 : 8, n_chunks = (cols - 1) / w + 1;
-    // enough workgroups for every CU to have two, but no part below 4 chunks a thread (two rounds of loads are latency alone)
+    // enough workgroups for every CU to have eight, but no part below 2 chunks a thread (300 x 50001 bf16: 32 us as with
+    // fewer, larger parts; 600 x 100000 f32: 54 us, with 512 workgroups 69)
     Part p = {1, n_chunks, nullptr, nullptr};
-    const long long most = std::min<long long>(kThreads, (n_chunks + 2 * kLongThreads - 1) / (2 * kLongThreads));
-    const long long want = rows >= 512 ? 1 : (512 + rows - 1) / rows;
+    const long long most = std::min<long long>(kThreads, (n_chunks + 2 * kThreads - 1) / (2 * kThreads));
+    const long long want = rows >= 2048 ? 1 : (2048 + rows - 1) / rows;
     const int parts = (int)std::max<long long>(1, std::min(most, want));
     p.chunks = (n_chunks - 1) / parts + 1;
     p.parts = (n_chunks - 1) / p.chunks + 1;
     return p;
 }
 
-// rows of up to this many chunks of 16 bytes lie in a wave's registers
-constexpr int kWaveChunks = 8 * 64;
+// Rows of up to this many chunks of 16 bytes lie in a wave's registers, a chunk to a lane; up to so many a wave streams its
+// row.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the register file full of
+// keys; 60000 x 1000 f32, k = 5: 74 and 101.)
+constexpr int kHeldChunks = 64, kWaveChunks = 8 * 64;
 
 size_t part_bytes(int rows, int cols, int k, int type)
 {
@@ -694,16 +712,15 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
     else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 4>(a, k, stream);
     else if (chunks <= kWaveChunks) {
         const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, kMaxBlocks);
-        if (chunks <= 64) score_wave_kernel<X, PROBS, 1><<<blocks, kThreads, 0, stream>>>(a);
-        else if (chunks <= 128) score_wave_kernel<X, PROBS, 2><<<blocks, kThreads, 0, stream>>>(a);
-        else if (chunks <= 256) score_wave_kernel<X, PROBS, 4><<<blocks, kThreads, 0, stream>>>(a);
-        else score_wave_kernel<X, PROBS, 8><<<blocks, kThreads, 0, stream>>>(a);
+        const Part p = {1, chunks, nullptr, nullptr};
+        if (chunks <= kHeldChunks) score_wave_kernel<X, PROBS><<<blocks, kThreads, 0, stream>>>(a);
+        else score_long_kernel<X, PROBS, 64><<<blocks, kThreads, 0, stream>>>(a, p);
     } else {
         Part p = parts_of(a.rows, a.cols, a.type);
         const size_t jobs = (size_t)a.rows * p.parts;
         p.stats = static_cast<float4 *>(a.workspace);
         p.keys = reinterpret_cast<u64 *>(p.stats + (p.parts > 1 ? jobs : 0));
-        score_long_kernel<X, PROBS, kLongThreads><<<(int)std::min<size_t>(jobs, kMaxBlocks), kLongThreads, 0, stream>>>(a, p);
+        score_long_kernel<X, PROBS, kThreads><<<(int)std::min<size_t>(jobs, kMaxBlocks), kThreads, 0, stream>>>(a, p);
         if (p.parts > 1) {
             if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
             score_join_kernel<X, PROBS><<<std::min(a.rows, kMaxBlocks), kThreads, 0, stream>>>(a, p);
