@@ -113,12 +113,23 @@ struct Row {
     __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - T / S; }
 };
 
-template <typename X, bool PROBS>
-__device__ __forceinline__ float label_score(const lcrc_score_args &a, const X *x, const Row<PROBS> &row, size_t at)
-{
-    const int c = a.labels[at];
-    return c < 0 ? 0.0f : c >= a.cols ? NAN : row.ln_p(to_f32(x[c]));
-}
+// A label of a row and its class's value, asked for before the row is worked on: two loads that wait for one another.
+struct Label {
+    int c;
+    float v;
+    bool wanted;
+    template <typename X>
+    __device__ __forceinline__ Label(const lcrc_score_args &a, const X *x, size_t r, int j) : wanted(a.logp && j < a.n_labels)
+    {
+        c = wanted ? a.labels[r * a.n_labels + j] : -1;
+        v = to_f32(x[c < 0 || c >= a.cols ? 0 : c]);
+    }
+    template <bool PROBS>
+    __device__ __forceinline__ void put(const lcrc_score_args &a, const Row<PROBS> &row, size_t r, int j) const
+    {
+        if (wanted) a.logp[r * a.n_labels + j] = c < 0 ? 0.0f : c >= a.cols ? NAN : row.ln_p(v);
+    }
+};
 __device__ __forceinline__ bool wants_top(const lcrc_score_args &a) { return a.k > 0 && (a.top_index || a.top_logp); }
 
 // ---- short rows: 16 lanes to a row ----
@@ -152,9 +163,7 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
         Chunk<X, W> raw[J];
 #pragma unroll
         for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((16 * j + lane) * W, cols - W));
-        // a lane's first label and its value: on their way while the row is worked on
-        const int label = a.logp && lane < a.n_labels ? a.labels[r * a.n_labels + lane] : -1;
-        const float labelled = to_f32(x[label < 0 || label >= cols ? 0 : label]);
+        const Label label(a, x, r, lane);
         // (all chunks but the last J are whole)
         const int last = (16 * (J - 1) + lane) * W, start = min(last, cols - W);
         const auto live = [&](int j, int i) { return j < J - 1 || start + i >= last; };
@@ -181,10 +190,9 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
         if constexpr (PROBS) least = reduce16(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
-        if (a.logp && lane < a.n_labels)
-            a.logp[r * a.n_labels + lane] = label < 0 ? 0.0f : label >= cols ? NAN : row.ln_p(labelled);
+        label.put(a, row, r, lane);
         if (a.logp && a.n_labels > 16)
-            for (int j = lane + 16; j < a.n_labels; j += 16) a.logp[r * a.n_labels + j] = label_score<X, PROBS>(a, x, row, r * a.n_labels + j);
+            for (int j = lane + 16; j < a.n_labels; j += 16) Label(a, x, r, j).put(a, row, r, j);
         if constexpr (K > 0) {
             double best[K];
 #pragma unroll
@@ -457,9 +465,7 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
     for (size_t r = (size_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); r < (size_t)a.rows; r += stride) {
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
         const Chunk<X, W> raw = load_chunk<X, W>(x + start);
-        // a lane's label and its value: on their way while the row is worked on
-        const int label = a.logp && lane < a.n_labels ? a.labels[r * a.n_labels + lane] : -1;
-        const float labelled = to_f32(x[label < 0 || label >= cols ? 0 : label]);
+        const Label label(a, x, r, lane);
         float least = 0.0f;
         Stats s = {0.0f, 0.0f, 0.0f};
         float most = raw[W - 1];                    // of the chunk, without what it shares with the one before
@@ -477,8 +483,7 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
         if constexpr (PROBS) least = reduce64(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
-        if (a.logp && lane < a.n_labels)
-            a.logp[r * a.n_labels + lane] = label < 0 ? 0.0f : label >= cols ? NAN : row.ln_p(labelled);
+        label.put(a, row, r, lane);
         if (!wants_top(a)) continue;
         if (row.bad) {
             if (lane < a.k) put_bad(a, r, lane);
@@ -516,6 +521,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
         const size_t r = job / p.parts;
         const int from = (int)(job - r * p.parts) * p.chunks, to = min(from + p.chunks, n_chunks);
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        const Label label(a, x, r, p.parts == 1 ? t : kScoreMaxLabels);
         Stats s = {kLowest, 0.0f, 0.0f};
         float least = 0.0f, most = -INFINITY, second = -INFINITY;       // the best chunk, and the best value of the others
         int most_at = -1;
@@ -574,7 +580,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
         const Row<PROBS> row(s, least < 0.0f);
         if (p.parts == 1) {
             if (a.entropy && t == 0) a.entropy[r] = row.entropy();
-            if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
+            label.put(a, row, r, t);
         } else if (t == 0) p.stats[job] = float4{s.m, s.S, s.T, least};
         if (!want_top) continue;
         if (row.bad) {
@@ -625,6 +631,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
     const int t = team.t;
     for (size_t r = blockIdx.x; r < (size_t)a.rows; r += gridDim.x) {
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
+        const Label label(a, x, r, t);
         Stats s = {kLowest, 0.0f, 0.0f};
         float least = 0.0f;
         if (t < p.parts) {                          // (parts <= kThreads)
@@ -635,7 +642,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
         s = team.template join<PROBS>(s, least);
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && t == 0) a.entropy[r] = row.entropy();
-        if (a.logp && t < a.n_labels) a.logp[r * a.n_labels + t] = label_score<X, PROBS>(a, x, row, r * a.n_labels + t);
+        label.put(a, row, r, t);
         if (!wants_top(a)) continue;
         if (row.bad) {
             if (t < a.k) put_bad(a, r, t);
@@ -677,9 +684,10 @@ Part parts_of(int rows, int cols, int type)
 }
 
 // Rows of up to this many chunks of 16 bytes lie in a wave's registers, a chunk to a lane; up to so many a wave streams its
-// row.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the register file full of
-// keys; 60000 x 1000 f32, k = 5: 74 and 101.)
-constexpr int kHeldChunks = 64, kWaveChunks = 8 * 64;
+// row, beyond it a workgroup.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the
+// register file full of keys; 60000 x 1000 f32, k = 5: 74 and 101.  20000 x 4096 f32, k = 8: by a wave 68 us, by a workgroup 109;
+// 12000 x 8192: 80 and 88.)
+constexpr int kHeldChunks = 64, kWaveChunks = 32 * 64;
 
 size_t part_bytes(int rows, int cols, int k, int type)
 {
