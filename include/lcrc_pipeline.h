@@ -245,7 +245,7 @@ int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, 
 int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *dst, int type, long long ld, void *hip_stream);
 
 /* y = act(x W^T + bias), x[rows][n_in] and W[n_out][n_in] (NeuralNet's layout, nn.cpp:702-740) in the 8-bit form: exact
- * products of the held values, added up in 32 bits.  (Where y has 16 or 8 bits the matrix instructions cut off, inside each
+ * products of the held values, added up in 32 bits.  (Where y has 16 bits the matrix instructions cut off, inside each
  * group of eight products, what lies 13 bits below the largest of them: at most 7 * 2^-13 of sum |x w|.)  x is a matrix in that form (LCRC_T_E4M3, ldx ignored) or is
  * put into it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32, f16 or bf16
  * rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
@@ -277,7 +277,8 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *args, void *hip_s
  * lcrc_set_merger_fp8: the merger of the systems that lcrc_create_system runs from memory (1BT_DCT, 1BT, 3BT and LCRC at any
  * other geometry than the shipped ones) with 8-bit operands: normalised inputs, weights and hidden activations in e4m3 with
  * a scale per 128, sums, biases, sigmoid, softmax and output transform as ever.  Opt-in: the operands keep 4 significant
- * bits, so posteriors are a few 1e-2 from those of the 32-bit nets.  The shipped LCRC shapes: LCRC_E_UNSUPPORTED. */
+ * bits, so posteriors lie around 1e-2 from those of the 32-bit nets (synthetic nets of 1500 hidden units: the largest
+ * difference of a frame 1.4e-2 on average, 6.8e-2 at most).  The shipped LCRC shapes: LCRC_E_UNSUPPORTED. */
 int lcrc_posteriors_scored(lcrc_ctx *ctx, const float *mel, const int *off, int n_utts, float *post, const int *labels, int n_labels,
                            int k, float *logp, float *entropy, int *top_index, float *top_logp);
 int lcrc_set_merger_fp8(lcrc_ctx *ctx, int enabled);

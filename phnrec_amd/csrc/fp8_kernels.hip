@@ -39,27 +39,28 @@ __device__ __forceinline__ int to_e4m3(float a, float b, float c, float d)
     return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
-// A lane's 32 values of one (row, block): scale over the row's four lanes, bytes, exponent.
-__device__ __forceinline__ i8 quantise(const float (&v)[32], int *exponent)
+// A lane's 32 values of one (row, block): scale over the row's four lanes, bytes, exponent.  A maximum skips NaN, and the
+// conversion keeps it; infinities, which do not count for the scale and become NaN, take a way of their own.
+__device__ __forceinline__ i8 quantise(float (&v)[32], int *exponent)
 {
-    float most = 0.0f;
+    const auto largest = [&] {
+        float most = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 32; j++) {
-        const float t = fabsf(v[j]);
-        most = fmaxf(most, t < INFINITY ? t : 0.0f);          // (NaN and infinities do not count)
+        for (int j = 0; j < 32; j++) most = fmaxf(most, fabsf(v[j]));
+        most = fmaxf(most, __shfl_xor(most, 16));
+        return fmaxf(most, __shfl_xor(most, 32));
+    };
+    float most = largest();
+    if (__any(most == INFINITY)) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = fabsf(v[j]) < INFINITY ? v[j] : NAN;
+        most = largest();
     }
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
     const int e = block_exponent(most);
     const float inv = pow2(-e);
     i8 q;
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
-        float s[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) s[r] = fabsf(v[4 * t + r]) < INFINITY ? v[4 * t + r] * inv : NAN;
-        q[t] = to_e4m3(s[0], s[1], s[2], s[3]);
-    }
+    for (int t = 0; t < 8; t++) q[t] = to_e4m3(v[4 * t] * inv, v[4 * t + 1] * inv, v[4 * t + 2] * inv, v[4 * t + 3] * inv);
     *exponent = e;
     return q;
 }
@@ -223,9 +224,11 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
 // another) they cut every product off 13 bits below the group's largest one before they add (measured, for the scaled and the
 // plain form alike: 2^16 + 3 * 2^3 comes out whole, of 2^16 + 3 * 7 the sevens are gone); the groups' sums are added in 32
 // bits.  That is up to 7 * 2^-13 of the products' absolute sum, 1.4e-5 relative on normal values: nothing beside a result
-// that is rounded to 16 or 8 bits (2^-8 .. 2^-11, 2^-4), too much for one in 32 bits.  So products with an f32 result turn
-// their operands into bf16 -- exact: 4 significant bits, the block's scale goes into bf16's exponent (v_cvt_scalef32_pk_bf16_fp8;
-// below 2^-126 it loses bits) -- and use the bf16 instruction, whose sums are f32 throughout: half the rate.
+// that is rounded to 16 bits (2^-8, 2^-11), too much for one in 32 bits -- and for one in 8, whose rounding turns 1.4e-5 into
+// a whole step, 2^-3, wherever it lies that near to a border: a net with hidden values in 8 bits and results in f16 was off by
+// 5.5e-4 of its results where sums in 32 bits leave 2.1e-4.  So products with such results turn their operands into bf16 --
+// exact: 4 significant bits, the block's scale goes into bf16's exponent (v_cvt_scalef32_pk_bf16_fp8; below 2^-126 it loses
+// bits) -- and use the bf16 instruction, whose sums are f32 throughout: half the rate.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
@@ -596,7 +599,7 @@ void split_launch(const Fp8ProductParams &p, const void *x, long long ldx, hipSt
 {
     const bool deep = p.n_in > 128 * 4;
     if (p.y_type == LCRC_T_E4M3) {
-        if constexpr (!EXACT) {
+        if constexpr (EXACT) {
             if (deep) split_launch<EXACT, X, 8, 1, 8>(p, x, ldx, stream);
             else split_launch<EXACT, X, 8, 1, 4>(p, x, ldx, stream);
         }
@@ -618,10 +621,11 @@ void split_launch(const Fp8ProductParams &p, const void *x, long long ldx, hipSt
     else if (p.n_out >= 16 * 512) split_launch<EXACT, X, 2, 1, 16>(p, x, ldx, stream);
     else split_launch<EXACT, X, 1, 1, 16>(p, x, ldx, stream);
 }
+bool sums_in_32_bits(const Fp8ProductParams &p) { return p.y_type == LCRC_T_F32 || p.y_type == LCRC_T_E4M3; }
 template <typename X>
 hipError_t split_by_sums(const Fp8ProductParams &p, const void *x, long long ldx, hipStream_t stream)
 {
-    if (p.y_type == LCRC_T_F32) split_launch<true, X>(p, x, ldx, stream);
+    if (sums_in_32_bits(p)) split_launch<true, X>(p, x, ldx, stream);
     else split_launch<false, X>(p, x, ldx, stream);
     return hipGetLastError();
 }
@@ -676,8 +680,8 @@ hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
     //   4096 x 8192 x 2048 bf16   256 x 128 (256 tiles) 86, 128 x 128 (512) 73, 128 x 64 100
     //   777 x 1999 x 2309 f16     128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
     // In short sums nothing is read often enough to count, and small tiles fill the card better:
-    //   8192 x 372 x 1500 in 8 bits  128 x 128 22.9, 128 x 64 19.4
-    const bool exact = p.y_type == LCRC_T_F32, longer = p.n_in > 512;
+    //   8192 x 372 x 1500 in 8 bits  128 x 128 26.5, 128 x 64 25.3
+    const bool exact = sums_in_32_bits(p), longer = p.n_in > 512;
     if (tiles(p, 128, 64) <= 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
     if (exact) {
         if (longer && tiles(p, 128, 128) >= 512) tile_launch<true, 8, 2, 1, 4>(p, stream);
