@@ -210,7 +210,8 @@ enum { LCRC_T_F32 = 0, LCRC_T_F16 = 1, LCRC_T_BF16 = 2, LCRC_T_E4M3 = 3 };
  *   top_index / top_logp    the k classes with the largest x in falling order, equal values by rising index, and their ln p
  * A class of p = 0 (logit -inf, posterior 0) has ln p = -inf and can be among the k best of a row that has no others.  In a
  * row in which no class is left (all -inf; all 0) every ln p is -inf, the entropy 0 and the best are classes 0 .. k-1.  A
- * NaN, a logit of +inf or a posterior that is negative or infinite makes the row's ln p and entropy NaN and its top_index -1.
+ * NaN, a logit of +inf, a posterior that is negative or infinite or a sum of posteriors beyond the range of 32 bits makes the
+ * row's ln p and entropy NaN and its top_index -1.
  * Sums in 32 bits.  Any output may be NULL. */
 enum { LCRC_SCORE_LOGITS = 0, LCRC_SCORE_PROBS = 1 };
 typedef struct lcrc_score_args {
@@ -245,10 +246,11 @@ int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, 
 int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *dst, int type, long long ld, void *hip_stream);
 
 /* y = act(x W^T + bias), x[rows][n_in] and W[n_out][n_in] (NeuralNet's layout, nn.cpp:702-740) in the 8-bit form: exact
- * products of the held values, added up in 32 bits.  (Where y has 16 bits the matrix instructions cut off, inside each
+ * products of the held values, added up in 32 bits.  (Blocks of scale 2^-127 may count as zeros.  Where y has 16 bits the matrix instructions cut off, inside each
  * group of eight products, what lies 13 bits below the largest of them: at most 7 * 2^-13 of sum |x w|.)  x is a matrix in that form (LCRC_T_E4M3, ldx ignored) or is
  * put into it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32, f16 or bf16
  * rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
+ * n_in <= 2^23; W, x and y hold at most 2^26 tiles of 16 rows x 128 columns.
  * LCRC_ACT_SIGMOID: 1 / (1 + exp(-v)); LCRC_ACT_FSIGMOID: the same with the reference's fast exponential (fexp.h:14-21),
  * which its trained nets expect.  y overlaps no input. */
 enum { LCRC_ACT_NONE = 0, LCRC_ACT_SIGMOID = 1, LCRC_ACT_FSIGMOID = 2 };

@@ -83,11 +83,12 @@ template <bool PROBS>
 __device__ __forceinline__ void add_value(float v, float m, float &S, float &T)
 {
     if constexpr (PROBS) {
-        // v_log_f32 flushes what is below 2^-126: scaled by 2^32 there
+        // v_log_f32 flushes what is below 2^-126: scaled by 2^32 there.  T in units of 256 ln 2, so that it leaves f32's range no
+        // sooner than S does.
         const bool small = v < 0x1p-126f;
-        const float l = __builtin_amdgcn_logf(small ? v * 0x1p32f : v) - (small ? 32.0f : 0.0f);
+        const float l = fmaf(__builtin_amdgcn_logf(small ? v * 0x1p32f : v), 0x1p-8f, small ? -32 * 0x1p-8f : 0.0f);
         S += v;
-        T += v > 0.0f ? v * l : 0.0f;               // (in units of ln 2: finish())
+        T += v > 0.0f ? v * l : 0.0f;
     } else {
         const float d = v - m;
         const float e = __builtin_amdgcn_exp2f(d * kLog2e);
@@ -95,9 +96,6 @@ __device__ __forceinline__ void add_value(float v, float m, float &S, float &T)
         T = fmaf(e, fmaxf(d, -1e30f), T);           // (0 * -inf)
     }
 }
-template <bool PROBS>
-__device__ __forceinline__ float finish(float T) { return PROBS ? T * kLn2 : T; }
-
 template <bool PROBS>
 struct Row {
     float m, S, T, ln_s;
@@ -110,7 +108,7 @@ struct Row {
         if (none) return -INFINITY;
         return (PROBS ? logf(v) : v - m) - ln_s;
     }
-    __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - T / S; }
+    __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - T / S * (PROBS ? 256.0f * kLn2 : 1.0f); }
 };
 
 // A label of a row and its class's value, asked for before the row is worked on: two loads that wait for one another.
@@ -189,7 +187,7 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
                 add_value<PROBS>(v, m, s.S, s.T);
             }
         s.S = reduce16(s.S, Add());
-        s.T = finish<PROBS>(reduce16(s.T, Add()));
+        s.T = reduce16(s.T, Add());
         if constexpr (PROBS) least = reduce16(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
@@ -483,7 +481,7 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
             add_value<PROBS>(v, s.m, s.S, s.T);
         }
         s.S = reduce64(s.S, Add());
-        s.T = finish<PROBS>(reduce64(s.T, Add()));
+        s.T = reduce64(s.T, Add());
         if constexpr (PROBS) least = reduce64(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
@@ -582,7 +580,6 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
         int c0 = from + t;
         for (; c0 - t + U * T <= whole; c0 += U * T) take(c0, std::false_type());
         for (; c0 < to; c0 += U * T) take(c0, std::true_type());
-        s.T = finish<PROBS>(s.T);
         s = team.template join<PROBS>(s, least);
         const Row<PROBS> row(s, least < 0.0f);
         if (p.parts == 1) {

@@ -7,7 +7,7 @@ import pytest
 
 from phnrec_amd import modelgen
 from tests import ops_ref as ref
-from tests.test_gpu_ops import Linear, Scored, _activations, _close, _stream, _weights
+from tests.test_gpu_ops import Linear, Scored, _activations, _close, _pack, _stream, _weights
 
 pytestmark = pytest.mark.gpu
 
@@ -255,3 +255,31 @@ def test_score_rows_made_against_the_search(capi, cols, k, shape):
     lp, en = ref.score_tolerance(exact, "logits")
     _close(got[3], want[3], lp[:, None])
     _close(got[1], want[1], en)
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("y_type", ["f32", "bf16", "e4m3"])
+def test_a_block_whose_scale_is_no_number(capi, y_type, rows):
+    """exponent byte 255 in one block of one row of W makes that output NaN, and no other"""
+    rng = np.random.default_rng(9)
+    n_in, n_out = 300, 70
+    q = torch.from_numpy(rng.integers(1, 120, (n_out, n_in)).astype(np.uint8)).cuda()
+    scales = np.full((n_out, 3), 120, np.uint8)
+    scales[33, 1] = 255
+    w = _pack(capi, q, "e4m3", n_out, n_in, n_in, torch.from_numpy(scales).cuda())
+    x = torch.from_numpy(_activations(rng, rows, n_in).astype(np.float32)).cuda()
+    got = Linear(capi, x, "f32", rows, n_in, n_out, w, None, "none", y_type).run().get()
+    want = np.zeros((rows, n_out), bool)
+    want[:, 33] = True
+    assert np.array_equal(np.isnan(got), want)
+
+
+@pytest.mark.parametrize("cols", [2, 300, 20000])
+def test_posteriors_whose_sum_leaves_the_range(capi, cols):
+    a = np.zeros((2, cols), np.float32)
+    a[0, :2] = 3e38
+    a[1, :2] = 1e38
+    x = torch.from_numpy(a).cuda()
+    logp, ent, ti, tl = Scored(capi, x, "f32", "probs", np.array([[0], [1]]), 2, cols).run().get()
+    assert np.isnan(logp[0]).all() and np.isnan(ent[0]) and (ti[0] == -1).all() and np.isnan(tl[0]).all()
+    assert abs(ent[1] - np.log(2)) < 1e-5 and ti[1].tolist() == [0, 1] and np.abs(tl[1] - np.log(0.5)).max() < 1e-4
