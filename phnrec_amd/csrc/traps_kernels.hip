@@ -776,45 +776,4 @@ hipError_t traps_1bt_launch(const MlpParams &p, hipStream_t stream, const char *
                            bt1_lds_plan((v->ks + 3) / 4, p.net.n_ot, ft, p.dct.trap_bands).total, stream);
 }
 
-// ---- softmax over rows in memory: the merger whose products ran in 8 bits (lcrc_set_merger_fp8) --------------------------
-// One wave per row, four rows per workgroup; a row's outputs in registers.
-template <int J>
-__global__ __launch_bounds__(256) void softmax_rows_kernel(const SoftmaxRowsParams p)
-{
-    const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= p.n_rows) return;
-    const float *in = p.in + row * p.n;
-    float v[J], m = -3.40282346638528859812e38f, sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < J; j++) {
-        v[j] = in[min(64 * j + lane, p.n - 1)];
-        m = fmaxf(m, v[j]);
-    }
-    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-#pragma unroll
-    for (int j = 0; j < J; j++) {
-        v[j] = 64 * j + lane < p.n ? fexp_nonpos_f(v[j] - m) : 0.0f;
-        sum += v[j];
-    }
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
-#pragma unroll
-    for (int j = 0; j < J; j++) {
-        float q = v[j] / sum;
-        q = soften(p.out_func[0], p.out_c[0], p.out_l[0], q);
-        q = soften(p.out_func[1], p.out_c[1], p.out_l[1], q);
-        if (p.out_be) q = __builtin_bit_cast(float, __builtin_bswap32(__builtin_bit_cast(unsigned, q)));
-        if (64 * j + lane < p.n) p.out[row * p.out_ld + 64 * j + lane] = q;
-    }
-}
-
-hipError_t softmax_rows_launch(const SoftmaxRowsParams &p, hipStream_t stream)
-{
-    const int blocks = (p.n_rows + 3) / 4;
-    if (p.n <= 256) softmax_rows_kernel<4><<<blocks, 256, 0, stream>>>(p);
-    else if (p.n <= 1024) softmax_rows_kernel<16><<<blocks, 256, 0, stream>>>(p);
-    else return hipErrorInvalidValue;
-    return hipGetLastError();
-}
-
 }  // namespace phnrec
