@@ -259,10 +259,20 @@ __device__ __forceinline__ unsigned bar_of(const unsigned (&v)[G], int k, int *r
 {
     unsigned res = 0;
     int n = 64 * G;
-    for (int bit = 31; bit >= 0 && n != k; bit--) {
-        const unsigned t = res | (1u << bit);
-        const int c = count_from(v, t);
-        if (c >= k) res = t, n = c;
+    if constexpr (G == 1) {
+        for (int bit = 31; bit >= 0 && n != k; bit--) {
+            const unsigned t = res | (1u << bit);
+            const int c = count_from(v, t);
+            if (c >= k) res = t, n = c;
+        }
+    } else {                                    // a workgroup waits for it: two bits at a time, three counts side by side
+        for (int bit = 30; bit >= 0 && n != k; bit -= 2) {
+            const unsigned t1 = res | (1u << bit), t2 = res | (2u << bit), t3 = res | (3u << bit);
+            const int c1 = count_from(v, t1), c2 = count_from(v, t2), c3 = count_from(v, t3);
+            if (c3 >= k) res = t3, n = c3;
+            else if (c2 >= k) res = t2, n = c2;
+            else if (c1 >= k) res = t1, n = c1;
+        }
     }
     *reached = n;
     return res;
@@ -655,16 +665,21 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
         // the parts' lists, rank by rank: the best ones lie with different threads; a key is a chunk of its own (its column)
         const u64 *keys = p.keys + r * p.parts * a.k;
         const int n = p.parts * a.k;
-        const auto key_at = [&](int i) { return keys[i % p.parts * a.k + i / p.parts]; };
-        u64 first[1] = {};
-#pragma unroll 8
-        for (int i = t; i < n; i += kThreads) first[0] = max(first[0], key_at(i));
-        const auto scan = [&](u64, const auto &f) {
+        // (kThreads keys further: so many ranks and lists further, without a division)
+        const int by_rank = kThreads / p.parts, by_list = kThreads % p.parts, rank0 = t / p.parts, list0 = t % p.parts;
+        const auto each = [&](const auto &f) {
+            int rank = rank0, list = list0;
 #pragma unroll 8
             for (int i = t; i < n; i += kThreads) {
-                const u64 key = key_at(i);
-                f(key != 0, key_value(key), key_column(key), key_column(key));
+                f(keys[list * a.k + rank]);
+                rank += by_rank, list += by_list;
+                if (list >= p.parts) list -= p.parts, rank++;
             }
+        };
+        u64 first[1] = {};
+        each([&](u64 key) { first[0] = max(first[0], key); });
+        const auto scan = [&](u64, const auto &f) {
+            each([&](u64 key) { f(key != 0, key_value(key), key_column(key), key_column(key)); });
         };
         team.top(a.k, first, scan, [&](const auto &f) { scan(0, f); }, [&](int rank, u64 key) { put_top<PROBS>(a, r, row, rank, key); });
     }
