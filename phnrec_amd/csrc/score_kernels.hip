@@ -60,6 +60,14 @@ __device__ __forceinline__ V reduce16(V v, Op op)
     v = op(v, dpp<0x122>(v));
     return op(v, dpp<0x121>(v));
 }
+// over 8 lanes: their pairs, their pairs of pairs, the two halves mirrored
+template <typename V, typename Op>
+__device__ __forceinline__ V reduce8(V v, Op op)
+{
+    v = op(v, dpp<0xb1>(v));                        // quad_perm 1 0 3 2, quad_perm 2 3 0 1, row_half_mirror
+    v = op(v, dpp<0x4e>(v));
+    return op(v, dpp<0x141>(v));
+}
 template <typename Op>
 __device__ __forceinline__ float reduce64(float v, Op op)
 {
@@ -130,7 +138,7 @@ struct Label {
 };
 __device__ __forceinline__ bool wants_top(const lcrc_score_args &a) { return a.k > 0 && (a.top_index || a.top_logp); }
 
-// ---- short rows: 16 lanes to a row ----
+// ---- short rows: 8 lanes to a row ----
 // A value and its column as ONE double: the f32 value (its conversion leaves 29 bits free) and the column in the free bits,
 // complemented where that makes the lower column the larger number.  So one v_max_f64, a full-rate instruction, orders values
 // and columns together, and a lane keeps its K best by K maxima and K - 1 minima for each value.  -inf sits at -2^200, below
@@ -178,25 +186,26 @@ __device__ __forceinline__ double settled(double a)
     return a;
 }
 
-// J chunks of W values to a lane: up to 16 J W columns; K: the longest list of best classes.
-// Bound by instructions: 524288 x 186 f32 with 3 best 107 us = 3.8 TB/s, a third of its 130 instructions a row f64 maxima and
-// what builds their operands (a wave to a row: 1680 us; rows prefetched by fewer, longer-lived workgroups: 114).  8192 x 138
-// with 5 best: 4 - 6 us.
+// J chunks of W values to a lane: up to 8 J W columns; K: the longest list of best classes.
+// Bound by instructions: 524288 x 186 f32 with 3 best 94 us = 4.3 TB/s, a third of its instructions f64 maxima and what builds their
+// operands (16 lanes to a row: 102 us; rows prefetched by fewer, longer-lived workgroups: slower by 10).  8192 x 138 with 5
+// best: 5.7 us.
 template <typename X, bool PROBS, int W, int J, int K>
 __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_args a)
 {
-    const int lane = threadIdx.x & 15, cols = a.cols;
-    const size_t stride = (size_t)gridDim.x * (kThreads / 16);
-    for (size_t r = (size_t)blockIdx.x * (kThreads / 16) + threadIdx.x / 16; r < (size_t)a.rows; r += stride) {
+    const int lane = threadIdx.x & 7, cols = a.cols;
+    const size_t stride = (size_t)gridDim.x * (kThreads / 8);
+    for (size_t r = (size_t)blockIdx.x * (kThreads / 8) + threadIdx.x / 8; r < (size_t)a.rows; r += stride) {
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
         Chunk<X, W> raw[J];
 #pragma unroll
-        for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((16 * j + lane) * W, cols - W));
+        for (int j = 0; j < J; j++) raw[j] = load_chunk<X, W>(x + min((8 * j + lane) * W, cols - W));
         const Label label(a, x, r, lane);
-        // (all chunks but the last J are whole)
-        const int last = (16 * (J - 1) + lane) * W, start = min(last, cols - W);
-        const auto live = [&](int j, int i) { return j < J - 1 || start + i >= last; };
-        const auto column = [&](int j, int i) { return (j < J - 1 ? (16 * j + lane) * W : start) + i; };
+        // (launch(): so many chunks of every lane are whole, the others may be cut off by the row's end or lie behind it)
+        constexpr int kWhole = J <= 4 ? J - 1 : J - 2;
+        const auto at = [&](int j) { return (8 * j + lane) * W; };
+        const auto live = [&](int j, int i) { return j < kWhole || min(at(j), cols - W) + i >= at(j); };
+        const auto column = [&](int j, int i) { return (j < kWhole ? at(j) : min(at(j), cols - W)) + i; };
         float m = kLowest, least = 0.0f;
         Stats s = {0.0f, 0.0f, 0.0f};
         if constexpr (!PROBS) {
@@ -204,7 +213,7 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
             for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < W; i++) m = fmaxf(m, raw[j][i]);       // (what is there twice does no harm)
-            s.m = m = reduce16(m, Max());
+            s.m = m = reduce8(m, Max());
         }
 #pragma unroll
         for (int j = 0; j < J; j++)
@@ -214,14 +223,14 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
                 if constexpr (PROBS) least = fminf(least, v);
                 add_value<PROBS>(v, m, s.S, s.T);
             }
-        s.S = reduce16(s.S, Add());
-        s.T = reduce16(s.T, Add());
-        if constexpr (PROBS) least = reduce16(least, Min());
+        s.S = reduce8(s.S, Add());
+        s.T = reduce8(s.T, Add());
+        if constexpr (PROBS) least = reduce8(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
         label.put(a, row, r, lane);
-        if (a.logp && a.n_labels > 16)
-            for (int j = lane + 16; j < a.n_labels; j += 16) Label(a, x, r, j).put(a, row, r, j);
+        if (a.logp && a.n_labels > 8)
+            for (int j = lane + 8; j < a.n_labels; j += 8) Label(a, x, r, j).put(a, row, r, j);
         if constexpr (K > 0) {
             double best[K];
 #pragma unroll
@@ -240,8 +249,8 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
                     }
                 }
             double mine = 0.0;
-            for (int n = 0; n < a.k; n++) {                  // the best head of the 16 lists, taken off its list
-                const double top = reduce16(settled(best[0]), Larger());
+            for (int n = 0; n < a.k; n++) {                  // the best head of the 8 lists, taken off its list
+                const double top = reduce8(settled(best[0]), Larger());
                 const bool won = best[0] == top;
 #pragma unroll
                 for (int q = 0; q < K; q++) best[q] = won ? (q + 1 < K ? best[q + 1] : -INFINITY) : best[q];
@@ -747,7 +756,7 @@ size_t part_bytes(int rows, int cols, int k, int type)
 template <typename X, bool PROBS, int W, int J>
 void launch_short(const lcrc_score_args &a, int k, hipStream_t stream)
 {
-    const int blocks = (int)std::min<long long>(((long long)a.rows + 15) / 16, kMaxBlocks);
+    const int blocks = (int)std::min<long long>(((long long)a.rows + kThreads / 8 - 1) / (kThreads / 8), kMaxBlocks);
     if (k == 0) score_short_kernel<X, PROBS, W, J, 0><<<blocks, kThreads, 0, stream>>>(a);
     else if (k == 1) score_short_kernel<X, PROBS, W, J, 1><<<blocks, kThreads, 0, stream>>>(a);
     else if (k <= 3) score_short_kernel<X, PROBS, W, J, 3><<<blocks, kThreads, 0, stream>>>(a);
@@ -761,10 +770,12 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
     constexpr int W = 16 / sizeof(X);
     const int k = a.top_index || a.top_logp ? a.k : 0, chunks = (a.cols - 1) / W + 1;
     if (a.cols < W) launch_short<X, PROBS, 1, 1>(a, k, stream);          // (k <= cols < 8)
-    else if (k <= 8 && chunks <= 16) launch_short<X, PROBS, W, 1>(a, k, stream);
-    else if (k <= 8 && chunks <= 32) launch_short<X, PROBS, W, 2>(a, k, stream);
-    else if (k <= 8 && chunks <= 48) launch_short<X, PROBS, W, 3>(a, k, stream);
-    else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 4>(a, k, stream);
+    else if (k <= 8 && chunks <= 8) launch_short<X, PROBS, W, 1>(a, k, stream);
+    else if (k <= 8 && chunks <= 16) launch_short<X, PROBS, W, 2>(a, k, stream);
+    else if (k <= 8 && chunks <= 24) launch_short<X, PROBS, W, 3>(a, k, stream);
+    else if (k <= 8 && chunks <= 32) launch_short<X, PROBS, W, 4>(a, k, stream);
+    else if (k <= 8 && chunks <= 48) launch_short<X, PROBS, W, 6>(a, k, stream);
+    else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 8>(a, k, stream);
     else if (chunks <= kWaveChunks) {
         const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, kMaxBlocks);
         const Part p = {1, chunks, nullptr, nullptr};
