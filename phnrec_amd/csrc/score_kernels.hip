@@ -673,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
     }
 }
 
-// joins the parts of each row.  All latency: 49 parts of 64 best 13 us, as much as the parts take (3 x 200003 f16).
+// joins the parts of each row.  All latency: 49 parts of 64 best 11 us, as much as the parts take (3 x 200003 f16).
 template <typename X, bool PROBS>
 __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_args a, const Part p)
 {

@@ -105,6 +105,19 @@ def test_score_against_64_bits(capi, rows, cols, k, m, pad, type, form):
     _check_scores(capi, _scores(rng, rows, cols, form), type, form, labels, k, pad)
 
 
+@pytest.mark.parametrize("form", ["probs", "logits"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("chunks", [1, 8, 16, 24, 32, 48, 64])
+def test_score_on_both_sides_of_a_rows_borders(capi, chunks, type, form):
+    """rows that end just before, at and just behind so many 16-byte chunks; more labels than lanes, a row more than a workgroup's"""
+    width = 4 if type == "f32" else 8
+    for cols in (chunks * width - 1, chunks * width, chunks * width + 1):
+        rng = np.random.default_rng(cols)
+        for k in (1, 2, 3, 5, 8):
+            if k <= cols:
+                _check_scores(capi, _scores(rng, 33, cols, form), type, form, rng.integers(-1, cols, (33, 19)), k, pad=k % 3)
+
+
 @pytest.mark.parametrize("cols", [3, 64, 138, 300, 1500, 5000, 40000])
 def test_score_ties_go_to_the_lowest_index(capi, cols):
     k = min(64, cols)
