@@ -1,7 +1,10 @@
 // lcrc_api_ops.cpp -- the operators on matrices in device memory behind the C ABI (include/lcrc_pipeline.h: lcrc_score,
 // lcrc_fp8_pack / _unpack / _linear): checks of arguments, the device of the call, launches.  No context, no allocation, no
-// wait; the kernels are in score_kernels.hip and fp8_kernels.hip.
+// wait; the kernels are in score_kernels.hip, fp8_kernels.hip and softmax_kernels.hip, an object that the first call loads.
 #include "lcrc_ctx.h"
+
+#include <dlfcn.h>
+
 #include "ops_dev.h"
 
 using namespace lcrc_impl;
@@ -26,6 +29,38 @@ struct DeviceScope {
         return LCRC_OK;
     }
 };
+
+// The kernels' object (ops_dev.h), which lies beside this library; NULL and a text where it cannot be had.  Loaded once, by the
+// first call that launches something, and never unloaded.
+const OpsTable *ops(std::string *why)
+{
+    struct Loaded {
+        const OpsTable *table = nullptr;
+        std::string error;
+        Loaded()
+        {
+            Dl_info here;
+            if (!dladdr(reinterpret_cast<const void *>(&lcrc_score), &here) || !here.dli_fname) { error = "cannot find this library's folder"; return; }
+            std::string path = here.dli_fname;
+            const size_t slash = path.rfind('/');
+            path = (slash == std::string::npos ? std::string() : path.substr(0, slash + 1)) + "libphnrec_lcrc_ops.so";
+            void *const object = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+            const auto table_of = object ? reinterpret_cast<const OpsTable *(*)()>(dlsym(object, "lcrc_ops_table")) : nullptr;
+            if (table_of) table = table_of();
+            else { const char *e = dlerror(); error = e ? e : path; }
+        }
+    };
+    static const Loaded loaded;
+    *why = loaded.error;
+    return loaded.table;
+}
+// ... for a call, with its error
+int kernels(lcrc_ctx *c, const OpsTable **table)
+{
+    std::string why;
+    *table = ops(&why);
+    return *table ? LCRC_OK : fail(c, LCRC_E_DEVICE, "cannot load the operators' kernels: " + why);
+}
 
 int element_bytes(int type) { return type == LCRC_T_F32 ? 4 : type == LCRC_T_E4M3 ? 1 : 2; }
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -81,10 +116,12 @@ int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, h
     }
     unsigned char *x = c->d_fp8, *h = x + x_bytes;
     float *y = reinterpret_cast<float *>(h + h_bytes);
+    const OpsTable *k;
+    if (const int rc = kernels(c, &k)) return rc;
     Fp8PackParams pack = {d_in, nullptr, LCRC_T_F32, n_rows, net.n_inp, net.n_inp, x, net.mean, net.dev};
-    HIP_TRY(c, fp8_pack_launch(pack, s));
-    HIP_TRY(c, fp8_product_launch({x, c->fp8_w1, net.b1, n_rows, net.n_inp, net.n_hid, LCRC_ACT_FSIGMOID, LCRC_T_E4M3, h, 0}, s));
-    HIP_TRY(c, fp8_product_launch({h, c->fp8_w2, net.b2, n_rows, net.n_hid, net.n_out, LCRC_ACT_NONE, LCRC_T_F32, y, net.n_out}, s));
+    HIP_TRY(c, k->fp8_pack(pack, s));
+    HIP_TRY(c, k->fp8_product({x, c->fp8_w1, net.b1, n_rows, net.n_inp, net.n_hid, LCRC_ACT_FSIGMOID, LCRC_T_E4M3, h, 0}, s));
+    HIP_TRY(c, k->fp8_product({h, c->fp8_w2, net.b2, n_rows, net.n_hid, net.n_out, LCRC_ACT_NONE, LCRC_T_F32, y, net.n_out}, s));
     SoftmaxRowsParams o;
     memset(&o, 0, sizeof o);
     o.in = y; o.out = m.out; o.out_ld = m.out_ld; o.n_rows = n_rows; o.n = net.n_out;
@@ -92,7 +129,7 @@ int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, h
     memcpy(o.out_c, m.out_c, sizeof o.out_c);
     memcpy(o.out_l, m.out_l, sizeof o.out_l);
     o.out_be = m.out_be;
-    HIP_TRY(c, softmax_rows_launch(o, s));
+    HIP_TRY(c, k->softmax_rows(o, s));
     return LCRC_OK;
 }
 
@@ -118,6 +155,8 @@ struct ScoreLayout {
 
 int scores_after(lcrc_ctx *c, const HostScores &w, int n_rows, const float *d_post)
 {
+    const OpsTable *kernel;
+    if (const int rc = kernels(c, &kernel)) return rc;
     const ScoreLayout l(c, w, n_rows);
     if (l.end > c->cap_scores) {
         if (c->d_scores) (void)hipFree(c->d_scores);
@@ -149,7 +188,7 @@ int scores_after(lcrc_ctx *c, const HostScores &w, int n_rows, const float *d_po
     a.top_index = w.k > 0 ? (int *)(d + l.index) : nullptr;
     a.top_logp = w.k > 0 ? (float *)(d + l.top) : nullptr;
     a.workspace = d + l.host_end; a.workspace_bytes = l.end - l.host_end;
-    HIP_TRY(c, score_launch(a, c->stream));
+    HIP_TRY(c, kernel->score(a, c->stream));
     HIP_TRY(c, hipMemcpyAsync(h + l.logp, d + l.logp, l.host_end - l.logp, hipMemcpyDeviceToHost, c->stream));
     return LCRC_OK;
 }
@@ -176,6 +215,8 @@ int lcrc_set_merger_fp8(lcrc_ctx *c, int enabled)
     if (c->system == SYS_LCRC)
         return fail(c, LCRC_E_UNSUPPORTED, "lcrc_set_merger_fp8: the fused LCRC kernels hold their operands in f32 or split f16");
     HIP_TRY(c, hipSetDevice(c->device));
+    const OpsTable *k;
+    if (const int rc = kernels(c, &k)) return rc;
     if (!c->fp8_w1) {
         const HostNet &net = c->model->host[2];
         for (const std::vector<float> *w : {&net.w1, &net.w2})
@@ -185,7 +226,7 @@ int lcrc_set_merger_fp8(lcrc_ctx *c, int enabled)
         void *w1 = nullptr, *w2 = nullptr, *rows = nullptr;
         const auto pack = [&](const std::vector<float> &w, int n_out, int n_in, void *dst) {
             if (const hipError_t e = hipMemcpy(rows, w.data(), w.size() * sizeof(float), hipMemcpyHostToDevice); e != hipSuccess) return e;
-            if (const hipError_t e = fp8_pack_launch({rows, nullptr, LCRC_T_F32, n_out, n_in, n_in, (unsigned char *)dst, nullptr, nullptr}, c->stream);
+            if (const hipError_t e = k->fp8_pack({rows, nullptr, LCRC_T_F32, n_out, n_in, n_in, (unsigned char *)dst, nullptr, nullptr}, c->stream);
                 e != hipSuccess) return e;
             return hipStreamSynchronize(c->stream);
         };
@@ -259,7 +300,9 @@ int lcrc_score(int device_id, const lcrc_score_args *a, void *hip_stream)
         return bad(call, "workspace missing, smaller than lcrc_score_workspace says or not aligned to 16 bytes");
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
-    return launched(call, score_launch(*a, static_cast<hipStream_t>(hip_stream)));
+    const OpsTable *k;
+    if (const int rc = kernels(nullptr, &k)) return rc;
+    return launched(call, k->score(*a, static_cast<hipStream_t>(hip_stream)));
 }
 
 size_t lcrc_fp8_bytes(int rows, int cols)
@@ -279,8 +322,10 @@ int lcrc_fp8_pack(int device_id, const void *src, int type, int rows, int cols, 
     if (const int rc = check_held(call, dst, rows, cols)) return rc;
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
+    const OpsTable *k;
+    if (const int rc = kernels(nullptr, &k)) return rc;
     const Fp8PackParams p = {src, scales, type, rows, cols, ld, static_cast<unsigned char *>(dst), nullptr, nullptr};
-    return launched(call, fp8_pack_launch(p, static_cast<hipStream_t>(hip_stream)));
+    return launched(call, k->fp8_pack(p, static_cast<hipStream_t>(hip_stream)));
 }
 
 int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *dst, int type, long long ld, void *hip_stream)
@@ -293,8 +338,10 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
     if (const int rc = check_held(call, src, rows, cols)) return rc;
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
+    const OpsTable *k;
+    if (const int rc = kernels(nullptr, &k)) return rc;
     const Fp8UnpackParams p = {static_cast<const unsigned char *>(src), type, rows, cols, ld, dst};
-    return launched(call, fp8_unpack_launch(p, static_cast<hipStream_t>(hip_stream)));
+    return launched(call, k->fp8_unpack(p, static_cast<hipStream_t>(hip_stream)));
 }
 
 size_t lcrc_fp8_linear_workspace(int rows, int n_in, int x_type)
@@ -325,16 +372,18 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
         return bad(call, "workspace missing, smaller than lcrc_fp8_linear_workspace says or not aligned to 16 bytes");
     DeviceScope device;
     if (const int rc = device.enter(device_id)) return rc;
+    const OpsTable *k;
+    if (const int rc = kernels(nullptr, &k)) return rc;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const unsigned char *x = a->x_type == LCRC_T_E4M3 ? static_cast<const unsigned char *>(a->x) : nullptr;
     Fp8ProductParams p = {x, static_cast<const unsigned char *>(a->w), a->bias, a->rows, a->n_in, a->n_out, a->act, a->y_type, a->y, a->ldy};
     if (a->x_type != LCRC_T_E4M3) {
-        if (a->rows <= kQRows && a->n_out <= kQFewOut) return launched(call, fp8_few_rows_launch(p, a->x, a->x_type, a->ldx, s));
+        if (a->rows <= kQRows && a->n_out <= kQFewOut) return launched(call, k->fp8_few_rows(p, a->x, a->x_type, a->ldx, s));
         const Fp8PackParams pack = {a->x, nullptr, a->x_type, a->rows, a->n_in, a->ldx, static_cast<unsigned char *>(a->workspace), nullptr, nullptr};
-        if (const int rc = launched(call, fp8_pack_launch(pack, s))) return rc;
+        if (const int rc = launched(call, k->fp8_pack(pack, s))) return rc;
         p.x = pack.dst;
     }
-    return launched(call, fp8_product_launch(p, s));
+    return launched(call, k->fp8_product(p, s));
 }
 
 }  // extern "C"

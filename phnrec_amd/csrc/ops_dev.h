@@ -1,14 +1,18 @@
 // ops_dev.h -- what the operators on matrices in device memory (include/lcrc_pipeline.h: lcrc_score, lcrc_fp8_*) share between
-// their C entries (lcrc_api_ops.cpp) and their kernels (score_kernels.hip, fp8_kernels.hip).
+// their C entries (lcrc_api_ops.cpp) and their kernels (score_kernels.hip, fp8_kernels.hip, softmax_kernels.hip).  The kernels
+// are a shared object of their own, libphnrec_lcrc_ops.so, which the first call that needs one of them loads: a process
+// that uses none of them -- the `phnrec` command line -- registers none with the HIP runtime.
 #ifndef PHNREC_OPS_DEV_H
 #define PHNREC_OPS_DEV_H
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 
 #include "../../include/lcrc_pipeline.h"
+#include "lcrc_dev.h"
 
 namespace phnrec {
 
@@ -16,8 +20,38 @@ namespace phnrec {
 constexpr int kScoreMaxTop = 64, kScoreMaxLabels = 64;
 constexpr int kScoreMaxCols = 1 << 30;
 
-size_t score_workspace_bytes(int rows, int cols, int k);
-hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream);
+// Rows of up to this many chunks of 16 bytes lie in a wave's registers, a chunk to a lane; up to so many a wave streams its
+// row, beyond it a workgroup.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the
+// register file full of keys; 60000 x 1000 f32, k = 5: 74 and 101.  20000 x 4096 f32, k = 8: by a wave 68 us, by a workgroup 109;
+// 12000 x 8192: 80 and 88.)
+constexpr int kScoreThreads = 256, kScoreHeldChunks = 64, kScoreWaveChunks = 32 * 64;
+
+// a row's cut into parts of so many chunks of 16 bytes, a workgroup to each
+struct ScoreParts {
+    int parts, chunks;
+};
+inline ScoreParts score_parts(int rows, int cols, int type)
+{
+    const int w = type == LCRC_T_F32 ? 4 : 8, n_chunks = (cols - 1) / w + 1;
+    // enough workgroups for every CU to have eight, but no part below 2 chunks a thread (300 x 50001 bf16: 32 us as with
+    // fewer, larger parts; 600 x 100000 f32: 54 us, with 512 workgroups 69)
+    const long long most = std::min<long long>(kScoreThreads, (n_chunks + 2 * kScoreThreads - 1) / (2 * kScoreThreads));
+    const long long want = rows >= 2048 ? 1 : (2048 + rows - 1) / rows;
+    const int parts = (int)std::max<long long>(1, std::min(most, want)), chunks = (n_chunks - 1) / parts + 1;
+    return {(n_chunks - 1) / chunks + 1, chunks};
+}
+// the parts' statistics (16 bytes) and lists of k keys, of either width of type: the size function does not take the type
+inline size_t score_workspace_bytes(int rows, int cols, int k)
+{
+    size_t most = 0;
+    for (const int type : {(int)LCRC_T_F32, (int)LCRC_T_BF16}) {
+        const int w = type == LCRC_T_F32 ? 4 : 8;
+        if ((cols - 1) / w + 1 <= kScoreWaveChunks) continue;
+        const ScoreParts p = score_parts(rows, cols, type);
+        if (p.parts > 1) most = std::max(most, (size_t)rows * p.parts * (16 + (size_t)k * 8));
+    }
+    return most;
+}
 
 // ---- the 8-bit matrix form ------------------------------------------------------------------------------------------
 // A matrix [rows][cols] in e4m3, rows in tiles of 16, columns in blocks of 128, in the order in which a lane of
@@ -60,14 +94,26 @@ struct Fp8ProductParams {
     void *y;
     long long ldy;
 };
+constexpr int kQFewOut = 1 << 25;     // outputs of a product that converts its rows itself
+constexpr long long kQMaxTiles = 1ll << 26;      // of a matrix in the 8-bit form, of x and of y (a grid holds 2^32 threads)
+constexpr int kQMaxIn = 1 << 23;      // columns of the operands of a product: their tiles' offsets stay within 32 bits
+
+// ---- the kernels' object ----------------------------------------------------------------------------------------------
+// Its one exported symbol, lcrc_ops_table, gives the launches.
+struct OpsTable {
+    hipError_t (*score)(const lcrc_score_args &a, hipStream_t stream);
+    hipError_t (*fp8_pack)(const Fp8PackParams &p, hipStream_t stream);
+    hipError_t (*fp8_unpack)(const Fp8UnpackParams &p, hipStream_t stream);
+    hipError_t (*fp8_product)(const Fp8ProductParams &p, hipStream_t stream);
+    // up to kQRows rows of f32, f16 or bf16: converted by the product itself (p.x is not read)
+    hipError_t (*fp8_few_rows)(const Fp8ProductParams &p, const void *x, int x_type, long long ldx, hipStream_t stream);
+    hipError_t (*softmax_rows)(const SoftmaxRowsParams &p, hipStream_t stream);
+};
+hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream);
 hipError_t fp8_pack_launch(const Fp8PackParams &p, hipStream_t stream);
 hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream);
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream);
-// up to kQRows rows of f32, f16 or bf16: converted by the product itself (p.x is not read)
 hipError_t fp8_few_rows_launch(const Fp8ProductParams &p, const void *x, int x_type, long long ldx, hipStream_t stream);
-constexpr int kQFewOut = 1 << 25;     // ... and up to this many outputs
-constexpr long long kQMaxTiles = 1ll << 26;      // of a matrix in the 8-bit form, of x and of y (a grid holds 2^32 threads)
-constexpr int kQMaxIn = 1 << 23;      // columns of the operands of a product: their tiles' offsets stay within 32 bits
 
 }  // namespace phnrec
 #endif

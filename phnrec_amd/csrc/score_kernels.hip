@@ -20,7 +20,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kScoreThreads;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.40282346638528859812e38f;
 
@@ -725,34 +725,6 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
 // ---- which kernel, on what grid ----
 constexpr int kMaxBlocks = 1 << 22;      // beyond it the workgroups take several rows each
 
-Part parts_of(int rows, int cols, int type)
-{
-    const int w = type == LCRC_T_F32 ? 4 : 8, n_chunks = (cols - 1) / w + 1;
-    // enough workgroups for every CU to have eight, but no part below 2 chunks a thread (300 x 50001 bf16: 32 us as with
-    // fewer, larger parts; 600 x 100000 f32: 54 us, with 512 workgroups 69)
-    Part p = {1, n_chunks, nullptr, nullptr};
-    const long long most = std::min<long long>(kThreads, (n_chunks + 2 * kThreads - 1) / (2 * kThreads));
-    const long long want = rows >= 2048 ? 1 : (2048 + rows - 1) / rows;
-    const int parts = (int)std::max<long long>(1, std::min(most, want));
-    p.chunks = (n_chunks - 1) / parts + 1;
-    p.parts = (n_chunks - 1) / p.chunks + 1;
-    return p;
-}
-
-// Rows of up to this many chunks of 16 bytes lie in a wave's registers, a chunk to a lane; up to so many a wave streams its
-// row, beyond it a workgroup.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the
-// register file full of keys; 60000 x 1000 f32, k = 5: 74 and 101.  20000 x 4096 f32, k = 8: by a wave 68 us, by a workgroup 109;
-// 12000 x 8192: 80 and 88.)
-constexpr int kHeldChunks = 64, kWaveChunks = 32 * 64;
-
-size_t part_bytes(int rows, int cols, int k, int type)
-{
-    const int w = type == LCRC_T_F32 ? 4 : 8;
-    if ((cols - 1) / w + 1 <= kWaveChunks) return 0;
-    const Part p = parts_of(rows, cols, type);
-    return p.parts == 1 ? 0 : (size_t)rows * p.parts * (sizeof(float4) + (size_t)k * sizeof(u64));
-}
-
 template <typename X, bool PROBS, int W, int J>
 void launch_short(const lcrc_score_args &a, int k, hipStream_t stream)
 {
@@ -776,16 +748,16 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
     else if (k <= 8 && chunks <= 32) launch_short<X, PROBS, W, 4>(a, k, stream);
     else if (k <= 8 && chunks <= 48) launch_short<X, PROBS, W, 6>(a, k, stream);
     else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 8>(a, k, stream);
-    else if (chunks <= kWaveChunks) {
+    else if (chunks <= kScoreWaveChunks) {
         const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, kMaxBlocks);
         const Part p = {1, chunks, nullptr, nullptr};
-        if (chunks <= kHeldChunks) score_wave_kernel<X, PROBS><<<blocks, kThreads, 0, stream>>>(a);
+        if (chunks <= kScoreHeldChunks) score_wave_kernel<X, PROBS><<<blocks, kThreads, 0, stream>>>(a);
         else score_long_kernel<X, PROBS, 64><<<blocks, kThreads, 0, stream>>>(a, p);
     } else {
-        Part p = parts_of(a.rows, a.cols, a.type);
-        const size_t jobs = (size_t)a.rows * p.parts;
-        p.stats = static_cast<float4 *>(a.workspace);
-        p.keys = reinterpret_cast<u64 *>(p.stats + (p.parts > 1 ? jobs : 0));
+        const ScoreParts cut = score_parts(a.rows, a.cols, a.type);
+        const size_t jobs = (size_t)a.rows * cut.parts;
+        float4 *const stats = static_cast<float4 *>(a.workspace);
+        const Part p = {cut.parts, cut.chunks, stats, reinterpret_cast<u64 *>(stats + (cut.parts > 1 ? jobs : 0))};
         score_long_kernel<X, PROBS, kThreads><<<(int)std::min<size_t>(jobs, kMaxBlocks), kThreads, 0, stream>>>(a, p);
         if (p.parts > 1) {
             if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -796,12 +768,6 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
 }
 
 }  // namespace
-
-size_t score_workspace_bytes(int rows, int cols, int k)
-{
-    // (of either width of type: the size function does not take the type)
-    return std::max(part_bytes(rows, cols, k, LCRC_T_F32), part_bytes(rows, cols, k, LCRC_T_BF16));
-}
 
 hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream)
 {

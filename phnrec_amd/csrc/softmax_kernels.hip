@@ -4,6 +4,7 @@
 
 #include "lcrc_dev.h"
 #include "mlp_dev.h"
+#include "ops_dev.h"
 
 namespace phnrec {
 
@@ -48,3 +49,11 @@ hipError_t softmax_rows_launch(const SoftmaxRowsParams &p, hipStream_t stream)
 }
 
 }  // namespace phnrec
+
+// the launches of this object (ops_dev.h)
+extern "C" __attribute__((visibility("default"))) const phnrec::OpsTable *lcrc_ops_table()
+{
+    static const phnrec::OpsTable table = {phnrec::score_launch, phnrec::fp8_pack_launch, phnrec::fp8_unpack_launch, phnrec::fp8_product_launch,
+                                           phnrec::fp8_few_rows_launch, phnrec::softmax_rows_launch};
+    return &table;
+}

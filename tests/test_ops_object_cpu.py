@@ -1,0 +1,44 @@
+"""The operators' kernels are an object of their own, which a process that uses none of them -- the command line -- never loads."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+from phnrec_amd import capi
+from tests.util import GOLD, ROOT, model_dir
+
+OBJECT = os.path.join(ROOT, "phnrec_amd", "lib", "libphnrec_lcrc_ops.so")
+KERNELS = (b"score_short_kernel", b"score_wave_kernel", b"score_long_kernel", b"score_join_kernel", b"fp8_pack_kernel", b"fp8_unpack_kernel",
+           b"fp8_tile_kernel", b"fp8_split_kernel", b"softmax_rows_kernel")
+
+
+def test_the_library_registers_none_of_the_operators_kernels():
+    lib = open(capi.LIB_PATH, "rb").read()
+    ops = open(OBJECT, "rb").read()
+    for name in KERNELS:
+        assert name not in lib and name in ops
+
+
+def test_the_object_finds_what_it_needs():
+    """all symbols bound at once, as the library loads it; the table is complete"""
+    capi.load()
+    table = C.CDLL(OBJECT, mode=os.RTLD_NOW).lcrc_ops_table
+    table.restype = C.POINTER(C.c_void_p * 6)
+    assert all(table().contents)
+
+
+def test_refusals_and_sizes_do_not_load_it():
+    code = ("from phnrec_amd import capi\n"
+            "capi.score_workspace(3, 200003, 64); capi.fp8_bytes(5, 5)\n"
+            "try: capi.score(capi.ScoreArgs(rows=-1))\n"
+            "except capi.LcrcError: pass\n"
+            "print('lcrc_ops' in open('/proc/self/maps').read())\n")
+    assert subprocess.check_output([sys.executable, "-c", code], cwd=ROOT, text=True).split()[-1] == "False"
+
+
+def test_the_command_line_does_not_load_it(tmp_path):
+    """a conversion that ends in front of the GPU"""
+    p = subprocess.run([os.path.join(ROOT, "phnrec_amd", "bin", "phnrec"), "-c", model_dir("PHN_HU_SPDAT_LCRC_N1500"), "-i",
+                        os.path.join(GOLD, "test.raw"), "-t", "par", "-o", str(tmp_path / "o")], env=dict(os.environ, LD_DEBUG="files"),
+                       capture_output=True, text=True)
+    assert p.returncode == 0 and "libphnrec_lcrc.so" in p.stderr and "lcrc_ops" not in p.stderr
