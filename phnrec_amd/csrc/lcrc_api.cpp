@@ -9,10 +9,7 @@
 // device: lcrc_api_decoder.cpp; what the three share: lcrc_ctx.h.)
 #include "lcrc_ctx.h"
 
-#include <sys/mman.h>
-
 #include <cstdint>
-#include <unordered_map>
 
 namespace lcrc_impl {
 
@@ -286,59 +283,15 @@ hipError_t dev_alloc(void **p, size_t bytes)
 // every hipHostGetDevicePointer here).  Without the flag the registration belongs to the device that was current at
 // allocation time only -- invisible on a one-GPU box.
 // device_reads: a buffer that kernels read in place (mapped into the device, coherent: never cached on the device side)
-// Large buffers (the posterior, feature and byte buffers of a list's launches: 5-60 MB each) are the process's own
-// 2 MiB-aligned anonymous memory with MADV_HUGEPAGE, touched, then registered with the runtime (hipHostRegister, mapped
-// and portable): pinning and mapping 2 MiB pages instead of 4 KiB ones takes a third of hipHostMalloc's time -- 3 x 40 MiB:
-// 10.7 against 32 ms; 6 x 40 MiB: 23 against 67 ms -- and the kernel tears such a process down 30-40 ms sooner after exit
-// (tools/ubench/pin_probe, profiles/r06_ab_runs.txt 6).  Where transparent huge pages are off the advice is a no-op and
-// the cost is hipHostMalloc's.  Small buffers, and any failure on the way, take hipHostMalloc.  pinned_free() knows which.
-namespace {
-struct PinnedRegion { void *map_base; size_t map_bytes; };
-std::mutex g_pinned_mu;
-std::unordered_map<void *, PinnedRegion> g_pinned;
-constexpr size_t kHugePage = 2u << 20, kHugeMin = 4u << 20;
-}  // namespace
-
+// (Memory that the process already has is never registered instead -- hipHostRegister of 2 MiB pages pins large buffers in a
+// third of the time --: machines that refuse a registration leave an error behind which a later, unrelated call can report.)
 hipError_t pinned_alloc(void **p, size_t bytes, bool device_reads)
 {
     *p = nullptr;
-    if (inject_alloc_failure()) return hipErrorOutOfMemory;
-#ifndef LCRC_PINNED_PLAIN
-    if (bytes >= kHugeMin) {
-        const size_t len = (bytes + kHugePage - 1) & ~(kHugePage - 1), map_bytes = len + kHugePage;
-        void *base = mmap(nullptr, map_bytes, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
-        if (base != MAP_FAILED) {
-            void *h = (void *)(((uintptr_t)base + kHugePage - 1) & ~(uintptr_t)(kHugePage - 1));
-            (void)madvise(h, len, MADV_HUGEPAGE);
-            for (size_t o = 0; o < len; o += 4096) ((volatile char *)h)[o] = 0;      // (the pages exist before they are pinned)
-            if (hipHostRegister(h, len, hipHostRegisterMapped | hipHostRegisterPortable) == hipSuccess) {
-                std::lock_guard<std::mutex> l(g_pinned_mu);
-                g_pinned[h] = PinnedRegion{base, map_bytes};
-                *p = h;
-                return hipSuccess;
-            }
-            (void)hipGetLastError();
-            (void)munmap(base, map_bytes);
-        }
-    }
-#endif
-    return hipHostMalloc(p, bytes, device_reads ? kPinnedMapped : kPinned);
+    return inject_alloc_failure() ? hipErrorOutOfMemory : hipHostMalloc(p, bytes, device_reads ? kPinnedMapped : kPinned);
 }
 
-hipError_t pinned_free(void *p)
-{
-    if (!p) return hipSuccess;
-    PinnedRegion r{nullptr, 0};
-    {
-        std::lock_guard<std::mutex> l(g_pinned_mu);
-        auto it = g_pinned.find(p);
-        if (it != g_pinned.end()) { r = it->second; g_pinned.erase(it); }
-    }
-    if (!r.map_base) return hipHostFree(p);
-    const hipError_t e = hipHostUnregister(p);
-    (void)munmap(r.map_base, r.map_bytes);
-    return e;
-}
+hipError_t pinned_free(void *p) { return p ? hipHostFree(p) : hipSuccess; }
 
 void free_frame_staging(lcrc_ctx *c)
 {

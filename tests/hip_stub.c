@@ -52,8 +52,6 @@ hipError_t hipMalloc(void **p, size_t n) { return get(p, n); }
 hipError_t hipFree(void *p) { return put(p); }
 hipError_t hipHostMalloc(void **p, size_t n, unsigned f) { (void)f; return get(p, n); }
 hipError_t hipHostFree(void *p) { return put(p); }
-hipError_t hipHostRegister(void *p, size_t n, unsigned f) { (void)p; (void)n; (void)f; PLAIN }
-hipError_t hipHostUnregister(void *p) { (void)p; PLAIN }
 hipError_t hipHostGetDevicePointer(void **d, void *h, unsigned f) { (void)f; enter(); *d = h; return leave(); }
 hipError_t hipMemcpy(void *d, const void *s, size_t n, int k) { (void)k; enter(); memcpy(d, s, n); return leave(); }
 hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, int k, void *q) { (void)k; (void)q; enter(); memcpy(d, s, n); return leave(); }

@@ -54,3 +54,9 @@ def test_a_context_is_not_created_beside_a_warm_up(stub, tmp_path, system):
     lib = os.path.join(ROOT, "phnrec_amd", "lib", "libphnrec_lcrc.so")
     out = subprocess.check_output([sys.executable, "-c", RUN, stub, lib, d, system], text=True).split()
     assert out[:4] == ["beside", "a", "load:", "0"] and int(out[5]) > 20, out
+
+
+def test_pinned_memory_is_allocated_and_never_registered():
+    for name in ("libphnrec_lcrc.so", "libphnrec_lcrc_ops.so"):
+        wanted = subprocess.check_output(["nm", "-D", "--undefined-only", os.path.join(ROOT, "phnrec_amd", "lib", name)], text=True)
+        assert "hipLaunchKernel" in wanted and "hipHostRegister" not in wanted and "hipHostUnregister" not in wanted
