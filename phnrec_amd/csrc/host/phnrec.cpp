@@ -267,7 +267,8 @@ int main(int argc, char **argv)
 #if defined(__SANITIZE_ADDRESS__) || defined(__SANITIZE_THREAD__) || defined(PHNREC_COVERAGE)
     return 0;                                // sanitizer / coverage builds report from exit handlers
 #else
-    if (getenv("LD_PRELOAD") || getenv("ROCP_TOOL_LIBRARIES") || getenv("HSA_TOOLS_LIB") || getenv("PHNREC_CLEAN_EXIT")) return 0;
+    const auto named = [](const char *e) { return e && *e; };
+    if (named(getenv("LD_PRELOAD")) || named(getenv("ROCP_TOOL_LIBRARIES")) || named(getenv("HSA_TOOLS_LIB")) || named(getenv("PHNREC_CLEAN_EXIT"))) return 0;
     _Exit(0);
 #endif
 }
