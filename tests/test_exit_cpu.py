@@ -23,3 +23,17 @@ def test_ordinary_exit_only_for_a_tool_that_is_named(tmp_path, name, value, ordi
     p = subprocess.run([BIN, "-c", model_dir("PHN_HU_SPDAT_LCRC_N1500"), "-i", os.path.join(GOLD, "test.raw"), "-t", "par", "-o",
                         str(tmp_path / "o")], env=dict(env, LD_DEBUG="files"), capture_output=True, text=True)
     assert p.returncode == 0 and ("calling fini" in p.stderr) == ordinary
+
+
+def test_a_crash_names_its_place(tmp_path):
+    """the signal ends the process as before, behind the objects and offsets it ended in"""
+    import signal
+    import time
+    fifo = str(tmp_path / "in.raw")
+    os.mkfifo(fifo)                                          # (a file that never opens: the process waits)
+    p = subprocess.Popen([BIN, "-c", model_dir("PHN_HU_SPDAT_LCRC_N1500"), "-i", fifo, "-t", "par", "-o", str(tmp_path / "o")],
+                         stderr=subprocess.PIPE, text=True)
+    time.sleep(0.5)
+    p.send_signal(signal.SIGSEGV)
+    err = p.communicate(timeout=60)[1]
+    assert p.returncode == -signal.SIGSEGV and "ended by a signal" in err and "phnrec" in err.split("at\n", 1)[1], (p.returncode, err)
