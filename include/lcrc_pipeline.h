@@ -22,10 +22,10 @@ extern "C" {
  * a first lcrc_create) and returns when they are up.  Thread-safe; meant to be called from a helper thread at program
  * start so that the caller's own initialisation -- configuration, the model files and their re-packing inside
  * lcrc_create, the first file's front-end -- overlaps with it (the CLI does, one thread per device it will use).  It also
- * brings the posterior kernels' code object onto the device (20-40 ms that a context's creation or first launch pays
- * otherwise).  The device's part of lcrc_create and lcrc_clone -- stream, weight upload -- waits for a warm-up or preload of the
- * same device that is under way, and these for it: start-up calls take turns.  Join the helper thread before the first launch.
- * No reference counterpart: the reference has no device to bring up. */
+ * brings the posterior kernels' code object onto the device (20-40 ms that a
+ * context's creation or first launch pays otherwise; beside the caller's
+ * lcrc_create -- stream, weight upload -- it costs nothing: a one-file `phnrec` run 0.15-0.24 s instead of 0.21-0.29 on
+ * the same boxes).  No reference counterpart: the reference has no device to bring up. */
 int lcrc_device_warmup(int device_id);
 /* The same for the other code objects of the library: the GPU front-end's and the device decoder's kernels (15-20 ms each that
  * the first waveform / decoder launch of the process pays otherwise: a list's first launch 0.02-0.05 -> 0.003 s).  For the

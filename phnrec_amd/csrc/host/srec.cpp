@@ -392,13 +392,6 @@ void SpeechRec::WarmUpGpuAsync(bool frontend, bool decoder)
         });
 }
 
-void SpeechRec::JoinWarmUp()
-{
-    std::lock_guard<std::mutex> l(warmup_mu_);
-    for (auto &t : warmup_)
-        if (t.joinable()) t.join();
-}
-
 SpeechRec::~SpeechRec()
 {
     JoinWarmUp();
@@ -532,9 +525,6 @@ int SpeechRec::BringUpContext(int idx, const ContextPlan &plan, std::string &err
         mark(base < 0 ? "ctx: create" : "ctx: clone");
         if (!(base < 0 ? t->Init(config_dir_.c_str()) : t->InitClone(*gpus_[(size_t)base]))) return failed(t->LastError() + "\n");
         mark("ctx: created");
-        // (the library lets context creation and warm-up take turns; what follows here -- uploads, first launches -- must not run
-        //  beside a helper thread that still loads code either)
-        JoinWarmUp();
         const std::string e = SetUpContext(*t);
         if (!e.empty()) return failed(e);
         mark("ctx: front-end set");

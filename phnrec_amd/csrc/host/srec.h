@@ -114,7 +114,7 @@ public:
     // frontend / decoder: the run will (or may) use the GPU front-end / the device decoder -- a list, or the flags given --:
     // their code objects are brought onto the devices too (lcrc_device_preload)
     void WarmUpGpuAsync(bool frontend = false, bool decoder = false);
-    void JoinWarmUp();
+    void JoinWarmUp() { for (auto &t : warmup_) if (t.joinable()) t.join(); }
     ~SpeechRec();
     // srec.cpp:1201-1244: "src[ \t]+tgt" or "src" (target derived)
     bool ProcessFileListLine(DataFormat in, DataFormat out, const std::string &line);
@@ -208,7 +208,6 @@ private:
     std::vector<int> gpu_devices_;                    // physical device of each logical GPU (PHNREC_DEVICE_MAP)
     std::unique_ptr<ThreadPool> pool_;
     std::vector<std::thread> warmup_;
-    std::mutex warmup_mu_;                            // (every context's worker waits for them)
     RunStats stats_;
     MelBanks mb_proto_;
 };

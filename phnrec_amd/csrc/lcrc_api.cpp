@@ -36,15 +36,6 @@ int fail(lcrc_ctx *c, int code, const std::string &msg)
 }
 
 
-// A device's start-up -- the runtime comes up, code objects are loaded (lcrc_device_warmup, lcrc_device_preload) -- and the
-// creation of contexts on it (stream, events, uploads) take turns: no thread makes its first calls on a device while another
-// one loads code there.  Contexts are created side by side as ever.
-std::shared_mutex &start_up_gate(int device)
-{
-    static std::shared_mutex gate[64];
-    return gate[(unsigned)device % 64];
-}
-
 // (the copy is queued on the context's stream: a synchronous hipMemcpy from pageable memory costs a fresh process twice as
 //  much -- 17 ms against 8 ms for the first 6.6 MB, tools/ubench/hip_upload -- and every later use of the buffer is
 //  ordered behind it on that stream anyway; the creating call synchronises once before it hands the context out)
@@ -1002,7 +993,6 @@ static int create_traps(lcrc_ctx **out, const char *model_dir, int sys, int nban
     }
 
     lcrc_ctx *c = nullptr;
-    std::shared_lock<std::shared_mutex> turn(start_up_gate(device_id));
     {
         int rc = open_context(&c, nbanks, device_id);
         if (rc) return rc;
@@ -1077,7 +1067,6 @@ static int create_traps(lcrc_ctx **out, const char *model_dir, int sys, int nban
 
 int lcrc_device_warmup(int device_id)
 {
-    std::unique_lock<std::shared_mutex> turn(start_up_gate(device_id));
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0)
         return fail(nullptr, LCRC_E_DEVICE, "no HIP device available (this library has no CPU path)");
@@ -1091,7 +1080,6 @@ int lcrc_device_warmup(int device_id)
 
 int lcrc_device_preload(int device_id, int what)
 {
-    std::unique_lock<std::shared_mutex> turn(start_up_gate(device_id));
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0)
         return fail(nullptr, LCRC_E_DEVICE, "no HIP device available (this library has no CPU path)");
@@ -1148,7 +1136,6 @@ int lcrc_create(lcrc_ctx **out, const char *model_dir, int nbanks, int trap_len,
     }
     trace.mark("pack (host)");
     lcrc_ctx *c = nullptr;
-    std::shared_lock<std::shared_mutex> turn(start_up_gate(device_id));
     {
         int rc = open_context(&c, nbanks, device_id);
         if (rc) return rc;
@@ -1207,7 +1194,6 @@ int lcrc_clone(lcrc_ctx **out, const lcrc_ctx *src)
     if (!out || !src) return fail(nullptr, LCRC_E_ARG, "lcrc_clone: NULL argument");
     *out = nullptr;
     lcrc_ctx *c = nullptr;
-    std::shared_lock<std::shared_mutex> turn(start_up_gate(src->device));
     {
         int rc = open_context(&c, src->nbanks, src->device);
         if (rc) return rc;

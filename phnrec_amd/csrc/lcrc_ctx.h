@@ -18,7 +18,6 @@
 #include <memory>
 #include <mutex>
 #include <pthread.h>
-#include <shared_mutex>
 #include <string>
 #include <thread>
 #include <time.h>
@@ -213,7 +212,6 @@ struct HostScores {
 int scores_after(lcrc_ctx *c, const HostScores &w, int n_rows, const float *d_post);
 void fetch_scores(lcrc_ctx *c, const HostScores &w, int n_rows);
 // ---- lcrc_api.cpp ----
-std::shared_mutex &start_up_gate(int device);
 hipError_t dev_alloc(void **p, size_t bytes);
 hipError_t pinned_alloc(void **p, size_t bytes, bool device_reads = false);
 hipError_t pinned_free(void *p);         // for anything pinned_alloc or hipHostMalloc handed out
