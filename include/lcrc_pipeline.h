@@ -18,19 +18,16 @@ extern "C" {
 #endif
 
 /* ---- device start-up ------------------------------------------------------------------------ */
-/* Optional: starts the HIP runtime and GPU `device_id`'s context (~0.2 s in a fresh process, by far the largest part of
- * a first lcrc_create) and returns when they are up.  Thread-safe; meant to be called from a helper thread at program
- * start so that the caller's own initialisation -- configuration, the model files and their re-packing inside
- * lcrc_create, the first file's front-end -- overlaps with it (the CLI does, one thread per device it will use).  It also
- * brings the posterior kernels' code object onto the device (20-40 ms that a
- * context's creation or first launch pays otherwise; beside the caller's
- * lcrc_create -- stream, weight upload -- it costs nothing: a one-file `phnrec` run 0.15-0.24 s instead of 0.21-0.29 on
- * the same boxes).  No reference counterpart: the reference has no device to bring up. */
+/* Optional: starts the HIP runtime and GPU `device_id`'s context (by far the largest part of a first lcrc_create in a fresh
+ * process), brings the posterior kernels' code object onto the device (20-40 ms that a context's creation or first launch pays
+ * otherwise) and returns when they are up.  Meant for the start of a program, BEFORE its other threads: memory that a thread
+ * takes from the system while another one brings the runtime up has been lost again before its first use.  A program that has
+ * threads by then makes this (or any first HIP call) while they rest.  No reference counterpart: the reference has no device
+ * to bring up. */
 int lcrc_device_warmup(int device_id);
 /* The same for the other code objects of the library: the GPU front-end's and the device decoder's kernels (15-20 ms each that
- * the first waveform / decoder launch of the process pays otherwise: a list's first launch 0.02-0.05 -> 0.003 s).  For the
- * helper thread that ran lcrc_device_warmup, when the run will use them -- a one-file run that does not is 10 ms sooner done
- * without (the loads compete with its one context's creation). */
+ * the first waveform / decoder launch of the process pays otherwise: a list's first launch 0.02-0.05 -> 0.003 s), when the run
+ * will use them. */
 enum { LCRC_PRELOAD_FRONTEND = 1, LCRC_PRELOAD_DECODER = 2 };
 int lcrc_device_preload(int device_id, int what);
 /* PCI address of GPU `device_id` ("0000:c1:00.0") into buf: lets a host that drives several GPUs place the threads of

@@ -601,7 +601,7 @@ hipError_t frontend_launch(const FrontendParams &p, hipStream_t stream)
 }
 
 // This file's code object onto the current device (the runtime loads a code object with the first launch of one of its
-// kernels: 15-20 ms that a list's first waveform launch paid; lcrc_device_warmup pays them on its helper thread instead)
+// kernels: 15-20 ms that a list's first waveform launch paid; lcrc_device_preload pays them ahead)
 hipError_t frontend_preload_code()
 {
     hipFuncAttributes a;

@@ -129,7 +129,6 @@ static void Die(const std::string &msg)
 {
     fprintf(stderr, "ERROR: %s", msg.c_str());
     if (msg.empty() || msg.back() != '\n') fputc('\n', stderr);
-    if (g_sr) g_sr->JoinWarmUp();         // never leave under a thread that is still inside the HIP runtime
     LeaveAtOnce(1);
     exit(1);
 }
@@ -258,14 +257,7 @@ int main(int argc, char **argv)
     g_sr = &SR;
     SR.SetVerbose(verbose);
     if (!config_dir) Die("Configuration directory is not set (-c)\n");
-    // a conversion through the posterior estimator will need the GPU: bring the HIP runtime up NOW, on a helper thread,
-    // while the configuration, the model files and the weights' re-packing are dealt with on this one
     SR.SetGpus(gpus);
-    // (a list takes the GPU front-end by itself, over four or more GPUs the device decoder too; one file keeps the host's unless
-    //  the flags say otherwise: the warm-up threads load those kernels' code objects only for runs that will launch them)
-    if ((input_file || file_list) && (int)iformat <= (int)dfParams && (int)oformat >= (int)dfPosteriors)
-        SR.WarmUpGpuAsync(iformat == dfWaveform && (gpu_fe || gpu_en || file_list != nullptr),
-                          oformat == dfStrings && (gpu_dec || (file_list != nullptr && gpus >= 4)));
     if (batch > 0) SR.SetBatchFrames(batch);
     if (threads > 0) SR.SetHostThreads(threads);
     if (gpu_fe && gpu_en) Die("-F and -E are two forms of the GPU front-end: give one\n");
@@ -284,6 +276,13 @@ int main(int argc, char **argv)
     if (wformat != WF_UNKNOWN) SR.SetWaveFormat(wformat);
     if (output_file && !input_file) Die("The input file is not specified (-i)\n");
     if (!((int)oformat > (int)iformat)) Die("Unsupported data conversion (-s, -t)\n");
+
+    // a conversion through the posterior estimator needs the GPU: the HIP runtime comes up here, while there is one thread
+    // (a list takes the GPU front-end by itself, over four or more GPUs the device decoder too; one file keeps the host's unless
+    //  the flags say otherwise: those kernels' code objects are loaded only for runs that will launch them)
+    if ((input_file || file_list) && (int)iformat <= (int)dfParams && (int)oformat >= (int)dfPosteriors)
+        SR.WarmUpGpu(iformat == dfWaveform && (gpu_fe || gpu_en || file_list != nullptr),
+                     oformat == dfStrings && (gpu_dec || (file_list != nullptr && gpus >= 4)));
 
     if (input_file) {
         std::string line = input_file;
@@ -312,7 +311,6 @@ int main(int argc, char **argv)
                 s.host_threads, s.contexts, SR.ModeString().c_str(), MaxRssMb(), RssKinds().c_str());
     }
     // every output file is closed by now
-    SR.JoinWarmUp();
     LeaveAtOnce(0);
     return 0;
 }

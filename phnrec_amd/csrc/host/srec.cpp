@@ -375,26 +375,17 @@ bool SpeechRec::DeviceMap(std::vector<int> &devices)
     return true;
 }
 
-void SpeechRec::WarmUpGpuAsync(bool frontend, bool decoder)
+void SpeechRec::WarmUpGpu(bool frontend, bool decoder)
 {
-    if (!warmup_.empty()) return;
     std::vector<int> devices;
     if (!DeviceMap(devices)) { err_.clear(); devices.assign(1, 0); }      // (a bad map is reported where the contexts are planned)
     std::sort(devices.begin(), devices.end());
     devices.erase(std::unique(devices.begin(), devices.end()), devices.end());
-    // one thread per distinct device: seven more HIP start-ups of 80-100 ms each would otherwise begin only when the
-    // list's workers create their contexts (failures surface in lcrc_create)
     const int what = (frontend ? LCRC_PRELOAD_FRONTEND : 0) | (decoder ? LCRC_PRELOAD_DECODER : 0);
-    for (int dev : devices)
-        warmup_.emplace_back([dev, what] {
-            (void)lcrc_device_warmup(dev);
-            if (what) (void)lcrc_device_preload(dev, what);
-        });
-}
-
-SpeechRec::~SpeechRec()
-{
-    JoinWarmUp();
+    for (int dev : devices) {                // (failures surface in lcrc_create)
+        (void)lcrc_device_warmup(dev);
+        if (what) (void)lcrc_device_preload(dev, what);
+    }
 }
 
 // Whether lcrc_frontend_configure would take this configuration (its own limits, restated: lin16 / A-law, frames of

@@ -109,13 +109,12 @@ public:
     // features bit for bit at a tenth of its CPU time
     void SetGpuEnergies(bool v) { gpu_energies_ = v; }
     // Starts the HIP runtime and the primary context of EVERY distinct device the run will use (SetGpus first: -g N,
-    // PHNREC_DEVICE_MAP) on helper threads, one per device (lcrc_device_warmup): ~0.1-0.2 s each that then overlap with
-    // Init(), the model files, their re-packing and each other.  Call it as early as the conversion is known to need the GPU.
+    // PHNREC_DEVICE_MAP), one after the other (lcrc_device_warmup), before the process has any thread but this one: where a
+    // thread took memory from the system while another one brought the runtime up, that memory has been lost again before its
+    // first use (weights being packed beside a start-up on a helper thread: a segmentation fault in one of some 200 processes).
     // frontend / decoder: the run will (or may) use the GPU front-end / the device decoder -- a list, or the flags given --:
     // their code objects are brought onto the devices too (lcrc_device_preload)
-    void WarmUpGpuAsync(bool frontend = false, bool decoder = false);
-    void JoinWarmUp() { for (auto &t : warmup_) if (t.joinable()) t.join(); }
-    ~SpeechRec();
+    void WarmUpGpu(bool frontend = false, bool decoder = false);
     // srec.cpp:1201-1244: "src[ \t]+tgt" or "src" (target derived)
     bool ProcessFileListLine(DataFormat in, DataFormat out, const std::string &line);
     bool ProcessFileList(DataFormat in, DataFormat out, const std::string &list, const std::string &mlf);
@@ -207,7 +206,6 @@ private:
     int fe_vector_size_ = 0, fe_vector_step_ = 1;    // melbanks/vector_size, vector_step (FrontendFramesOf)
     std::vector<int> gpu_devices_;                    // physical device of each logical GPU (PHNREC_DEVICE_MAP)
     std::unique_ptr<ThreadPool> pool_;
-    std::vector<std::thread> warmup_;
     RunStats stats_;
     MelBanks mb_proto_;
 };

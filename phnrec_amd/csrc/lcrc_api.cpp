@@ -1125,8 +1125,7 @@ int lcrc_create(lcrc_ctx **out, const char *model_dir, int nbanks, int trap_len,
         if (ncoef != kNCoef) return create_traps(out, model_dir, SYS_LCRC_GEN, nbanks, trap_len, add_c0, 0, device_id);
     }
     trace.mark("model files");
-    // fragment order on the host first (no GPU involved: a caller that started lcrc_device_warmup on another thread has
-    // the HIP runtime coming up meanwhile), the three nets side by side
+    // fragment order on the host first (no GPU involved), the three nets side by side
     PackedNet packed[3];
     {
         std::thread t1([&] { pack_net_host(nets[1], packed[1]); }), t2([&] { pack_net_host(nets[2], packed[2]); });

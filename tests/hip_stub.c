@@ -2,6 +2,8 @@
  * device memory is host memory, copies are done at once, kernels do nothing.  Every call sleeps as long as stub_sleep_us says
  * for its kind and notes which other calls were inside the runtime meanwhile. */
 #define _GNU_SOURCE
+#include <dirent.h>
+#include <pthread.h>
 #include <stdatomic.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -15,8 +17,35 @@ atomic_int stub_inside, stub_loading, stub_beside_a_load, stub_calls, stub_launc
 int stub_load_us = 0;
 atomic_long stub_allocated;
 
+static int threads_of_this_process(void)
+{
+    int n = 0;
+    DIR *d = opendir("/proc/self/task");
+    for (struct dirent *e; d && (e = readdir(d));) n += e->d_name[0] != '.';
+    if (d) closedir(d);
+    return n;
+}
+/* the runtime comes up with the first call: it takes its time, and says how many threads the process has meanwhile */
+static void start_up(void)
+{
+    static pthread_mutex_t mu = PTHREAD_MUTEX_INITIALIZER;
+    static int up;
+    pthread_mutex_lock(&mu);
+    if (!up && getenv("STUB_START_UP")) {
+        int most = threads_of_this_process();
+        for (int i = 0; i < 20; i++) {
+            usleep(5000);
+            const int n = threads_of_this_process();
+            most = n > most ? n : most;
+        }
+        fprintf(stderr, "stub: %d thread(s) while the runtime comes up\n", most);
+    }
+    up = 1;
+    pthread_mutex_unlock(&mu);
+}
 static void enter(void)
 {
+    start_up();
     atomic_fetch_add(&stub_calls, 1);
     atomic_fetch_add(&stub_inside, 1);
     if (atomic_load(&stub_loading)) atomic_fetch_add(&stub_beside_a_load, 1);
