@@ -53,6 +53,9 @@ int lcrc_debug_fail_alloc(int nth);
 /* The same for launches: the nth (0 = next) posterior launch of this process from now on fails with LCRC_E_DEVICE before
  * anything is queued -- a device that refuses work in the middle of a list (tests of the callers' error paths). */
 int lcrc_debug_fail_launch(int nth);
+/* Bytes of this process's pinned buffers that its resident set does not count: a driver that backs pinned memory with objects
+ * of its own instead of the process's pages leaves all of them out (phnrec's PHNREC_STATS adds them to max_rss_mb). */
+long long lcrc_debug_pinned_outside_rss(void);
 
 #ifdef __cplusplus
 }

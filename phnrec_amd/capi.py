@@ -22,7 +22,7 @@ SYMBOLS = [
     "lcrc_reserve", "lcrc_wave_stage_buffer", "lcrc_wave_stage_run", "lcrc_wave_stage_energies", "lcrc_staged_posteriors",
     "lcrc_output_configure", "lcrc_decoder_configure", "lcrc_set_posterior_readback", "lcrc_last_labels", "lcrc_set_decoder_overlap", "lcrc_prev_labels", "lcrc_set_launch_order",
     "lcrc_reset", "lcrc_push", "lcrc_delay",
-    "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_kernel_name",
+    "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_debug_pinned_outside_rss", "lcrc_kernel_name",
     "lcrc_score_workspace", "lcrc_score", "lcrc_fp8_bytes", "lcrc_fp8_pack", "lcrc_fp8_unpack", "lcrc_fp8_linear_workspace", "lcrc_fp8_linear",
     "lcrc_posteriors_scored", "lcrc_set_merger_fp8",
 ]
@@ -182,6 +182,7 @@ def load():
     L.lcrc_set_arithmetic.argtypes = [vp, C.c_int]
     L.lcrc_debug_fail_alloc.argtypes = [C.c_int]
     L.lcrc_debug_fail_launch.argtypes = [C.c_int]
+    L.lcrc_debug_pinned_outside_rss.restype = C.c_longlong
     L.lcrc_posteriors_rows.argtypes = [vp, _f32p, C.c_int, C.c_int, C.c_int, _f32p]
     L.lcrc_score_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
     L.lcrc_score.argtypes = [C.c_int, C.POINTER(ScoreArgs), vp]

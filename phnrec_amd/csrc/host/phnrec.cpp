@@ -80,10 +80,12 @@ static int NextOpt(int argc, char **argv, const char *options, int &ind, const c
 static SpeechRec *g_sr = nullptr;
 
 // peak resident set of this process so far (PHNREC_STATS prints it: pinned buffers count)
+// (pinned buffers included, also where the resident set does not count them; they are as large as they ever were, since the
+// contexts are still there)
 static double MaxRssMb()
 {
     struct rusage ru;
-    return getrusage(RUSAGE_SELF, &ru) == 0 ? ru.ru_maxrss / 1024.0 : 0.0;
+    return (getrusage(RUSAGE_SELF, &ru) == 0 ? ru.ru_maxrss / 1024.0 : 0.0) + lcrc_debug_pinned_outside_rss() / 1048576.0;
 }
 
 // the resident set as it stands, by kind (/proc/self/status: RssAnon, RssFile, RssShmem), for PHNREC_STATS

@@ -10,6 +10,7 @@
 #include "lcrc_ctx.h"
 
 #include <cstdint>
+#include <unordered_map>
 
 namespace lcrc_impl {
 
@@ -276,13 +277,32 @@ hipError_t dev_alloc(void **p, size_t bytes)
 // device_reads: a buffer that kernels read in place (mapped into the device, coherent: never cached on the device side)
 // (Memory that the process already has is never registered instead -- hipHostRegister of 2 MiB pages pins large buffers in a
 // third of the time --: machines that refuse a registration leave an error behind which a later, unrelated call can report.)
+namespace {
+std::mutex g_pinned_mu;
+std::unordered_map<char *, size_t> g_pinned;         // the live buffers (lcrc_debug_pinned_outside_rss)
+}  // namespace
+
 hipError_t pinned_alloc(void **p, size_t bytes, bool device_reads)
 {
     *p = nullptr;
-    return inject_alloc_failure() ? hipErrorOutOfMemory : hipHostMalloc(p, bytes, device_reads ? kPinnedMapped : kPinned);
+    if (inject_alloc_failure()) return hipErrorOutOfMemory;
+    const hipError_t e = hipHostMalloc(p, bytes, device_reads ? kPinnedMapped : kPinned);
+    if (e == hipSuccess) {
+        std::lock_guard<std::mutex> l(g_pinned_mu);
+        g_pinned[static_cast<char *>(*p)] = bytes;
+    }
+    return e;
 }
 
-hipError_t pinned_free(void *p) { return p ? hipHostFree(p) : hipSuccess; }
+hipError_t pinned_free(void *p)
+{
+    if (!p) return hipSuccess;
+    {
+        std::lock_guard<std::mutex> l(g_pinned_mu);
+        g_pinned.erase(static_cast<char *>(p));
+    }
+    return hipHostFree(p);
+}
 
 void free_frame_staging(lcrc_ctx *c)
 {
@@ -1563,6 +1583,27 @@ int lcrc_posteriors_rows(lcrc_ctx *c, const float *mel, int n_rows, int row_firs
     HIP_TRY(c, wait_stream(c));
     memcpy(post, c->h_post, (size_t)row_count * O * sizeof(float));
     return LCRC_OK;
+}
+
+long long lcrc_debug_pinned_outside_rss(void)
+{
+    std::lock_guard<std::mutex> l(g_pinned_mu);
+    FILE *f = fopen("/proc/self/smaps", "r");
+    if (!f) return 0;
+    double outside = 0.0;
+    unsigned long from = 0, to = 0, kb = 0;
+    char line[512];
+    while (fgets(line, sizeof line, f)) {
+        unsigned long a, b;
+        if (sscanf(line, "%lx-%lx ", &a, &b) == 2) from = a, to = b;
+        else if (sscanf(line, "Rss: %lu kB", &kb) == 1 && to > from)
+            for (const auto &p : g_pinned) {          // (a mapping's resident part: taken as spread evenly over it)
+                const unsigned long lo = std::max(from, (unsigned long)p.first), hi = std::min(to, (unsigned long)p.first + p.second);
+                if (lo < hi) outside += (double)(hi - lo) * (1.0 - std::min(1.0, kb * 1024.0 / (double)(to - from)));
+            }
+    }
+    fclose(f);
+    return (long long)outside;
 }
 
 int lcrc_debug_fail_alloc(int nth)

@@ -8,6 +8,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
+#include <sys/mman.h>
 #include <unistd.h>
 
 typedef struct { unsigned x, y, z; } dim3;
@@ -79,8 +80,27 @@ static hipError_t put(void *p)
 }
 hipError_t hipMalloc(void **p, size_t n) { return get(p, n); }
 hipError_t hipFree(void *p) { return put(p); }
-hipError_t hipHostMalloc(void **p, size_t n, unsigned f) { (void)f; return get(p, n); }
-hipError_t hipHostFree(void *p) { return put(p); }
+/* pinned: mappings of their own, a page that holds the length in front, pages that nobody may touch around them */
+hipError_t hipHostMalloc(void **p, size_t n, unsigned f)
+{
+    (void)f;
+    enter();
+    const size_t len = (n + 4095) / 4096 * 4096;
+    char *m = mmap(0, len + 12288, PROT_NONE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+    mprotect(m, 4096, PROT_READ | PROT_WRITE);
+    *(size_t *)m = len + 12288;
+    mprotect(m, 4096, PROT_READ);
+    mprotect(m + 4096, 4096, PROT_NONE);
+    mprotect(m + 8192, len, PROT_READ | PROT_WRITE);
+    *p = m + 8192;
+    return leave();
+}
+hipError_t hipHostFree(void *p)
+{
+    enter();
+    if (p) munmap((char *)p - 8192, *(size_t *)((char *)p - 8192));
+    return leave();
+}
 hipError_t hipHostGetDevicePointer(void **d, void *h, unsigned f) { (void)f; enter(); *d = h; return leave(); }
 hipError_t hipMemcpy(void *d, const void *s, size_t n, int k) { (void)k; enter(); memcpy(d, s, n); return leave(); }
 hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, int k, void *q) { (void)k; (void)q; enter(); memcpy(d, s, n); return leave(); }

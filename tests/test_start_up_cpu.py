@@ -1,6 +1,7 @@
 """What the library and the command line do around the HIP runtime's start-up (on a stand-in runtime, hip_stub.c)."""
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -35,3 +36,33 @@ def test_pinned_memory_is_allocated_and_never_registered():
     for name in ("libphnrec_lcrc.so", "libphnrec_lcrc_ops.so"):
         wanted = subprocess.check_output(["nm", "-D", "--undefined-only", os.path.join(ROOT, "phnrec_amd", "lib", name)], text=True)
         assert "hipLaunchKernel" in wanted and "hipHostRegister" not in wanted and "hipHostUnregister" not in wanted
+
+
+OUTSIDE = """
+import ctypes as C, sys
+C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+L = C.CDLL(sys.argv[2])
+L.lcrc_stage_buffers.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
+c, a, b = C.c_void_p(), C.c_void_p(), C.c_void_p()
+L.lcrc_debug_pinned_outside_rss.restype = C.c_longlong
+assert L.lcrc_create(C.byref(c), sys.argv[3].encode(), 15, 31, 1, 0) == 0
+before = L.lcrc_debug_pinned_outside_rss()
+assert L.lcrc_stage_buffers(c, 100000, C.byref(a), C.byref(b)) == 0
+untouched = L.lcrc_debug_pinned_outside_rss()
+C.memmove(a, bytes(100000 * 15 * 4), 100000 * 15 * 4)
+C.memmove(b, bytes(100000 * 4), 100000 * 4)
+touched = L.lcrc_debug_pinned_outside_rss()
+L.lcrc_destroy.argtypes = [C.c_void_p]
+L.lcrc_destroy(c)
+print(before, untouched, touched, L.lcrc_debug_pinned_outside_rss())
+"""
+
+
+def test_pinned_memory_that_the_resident_set_leaves_out(stub, tmp_path):
+    """(memory that was never touched stands for memory that is not counted)"""
+    from phnrec_amd import capi, modelgen
+    modelgen.write_model_dir(str(tmp_path), 15, 64, 138, seed=3)
+    out = subprocess.check_output([sys.executable, "-c", OUTSIDE, stub, capi.LIB_PATH, str(tmp_path)], text=True)
+    before, untouched, touched, after = (int(v) for v in out.split())
+    rows = 100000 * 15 * 4
+    assert before < 1 << 20 and untouched >= rows * 0.9 and untouched - touched >= rows * 0.9 and after == 0, out
