@@ -83,25 +83,29 @@ struct Add { __device__ __forceinline__ float operator()(float a, float b) const
 
 // ---- a row's statistics ----
 struct Stats {
-    float m, S, T;      // S is NaN or inf in a row that is no distribution
+    float m, S, T;      // S is NaN or inf in a row that is no distribution; m: logits: the maximum, posteriors: T of small values
 };
 
-// the sums over one value; m: the row's (or the running) maximum
+// the sums over one value (logits: m is the row's or the running maximum)
 template <bool PROBS>
-__device__ __forceinline__ void add_value(float v, float m, float &S, float &T)
+__device__ __forceinline__ void add_value(float v, Stats &s)
 {
     if constexpr (PROBS) {
-        // v_log_f32 flushes what is below 2^-126: scaled by 2^32 there.  T in units of 256 ln 2, so that it leaves f32's range no
-        // sooner than S does.
-        const bool small = v < 0x1p-126f;
-        const float l = fmaf(__builtin_amdgcn_logf(small ? v * 0x1p32f : v), 0x1p-8f, small ? -32 * 0x1p-8f : 0.0f);
-        S += v;
-        T += v > 0.0f ? v * l : 0.0f;
+        // Both ends of f32's range: T is kept in units of 256 ln 2, so that it leaves the range no sooner than S does, and apart
+        // for values below 2^-64, times 2^64: their products would be subnormal, rounded to a multiple of 2^-149 (a row of 100
+        // values of 1e-45 had an entropy of 79 instead of 4.6).  The scaling also keeps v_log_f32 off what it flushes.
+        const bool small = v < 0x1p-64f;
+        const float w = small ? v * 0x1p64f : v;
+        const float l = fmaf(__builtin_amdgcn_logf(w), 0x1p-8f, small ? -64 * 0x1p-8f : 0.0f);
+        const float t = v > 0.0f ? w * l : 0.0f;
+        s.S += v;
+        s.T += small ? 0.0f : t;
+        s.m += small ? t : 0.0f;
     } else {
-        const float d = v - m;
+        const float d = v - s.m;
         const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-        S += e;
-        T = fmaf(e, fmaxf(d, -1e30f), T);           // (0 * -inf)
+        s.S += e;
+        s.T = fmaf(e, fmaxf(d, -1e30f), s.T);       // (0 * -inf)
     }
 }
 template <bool PROBS>
@@ -116,7 +120,7 @@ struct Row {
         if (none) return -INFINITY;
         return (PROBS ? logf(v) : v - m) - ln_s;
     }
-    __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - (PROBS ? T / S * (256.0f * kLn2) : T * __builtin_amdgcn_rcpf(S)); }
+    __device__ __forceinline__ float entropy() const { return bad ? NAN : none ? 0.0f : ln_s - (PROBS ? (T / S + m / (S * 0x1p64f)) * (256.0f * kLn2) : T * __builtin_amdgcn_rcpf(S)); }
 };
 
 // A label of a row and its class's value, asked for before the row is worked on: two loads that wait for one another.
@@ -221,11 +225,11 @@ __global__ __launch_bounds__(kThreads) void score_short_kernel(const lcrc_score_
             for (int i = 0; i < W; i++) {
                 const float v = live(j, i) ? raw[j][i] : PROBS ? 0.0f : -INFINITY;
                 if constexpr (PROBS) least = fminf(least, v);
-                add_value<PROBS>(v, m, s.S, s.T);
+                add_value<PROBS>(v, s);
             }
         s.S = reduce8(s.S, Add());
         s.T = reduce8(s.T, Add());
-        if constexpr (PROBS) least = reduce8(least, Min());
+        if constexpr (PROBS) s.m = reduce8(s.m, Add()), least = reduce8(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
         label.put(a, row, r, lane);
@@ -368,7 +372,8 @@ struct Team {
                 v.S *= f;
             }
         };
-        all.m = PROBS ? 0.0f : reduce64(s.m, Max());
+        if constexpr (PROBS) all.m = reduce64(s.m, Add());
+        else all.m = reduce64(s.m, Max());
         moved(s, all.m);
         all.S = reduce64(s.S, Add());
         all.T = reduce64(s.T, Add());
@@ -381,7 +386,7 @@ struct Team {
             }
             sync();
             float m = sh.slot[0];
-            for (int w = 1; w < kWaves; w++) m = fmaxf(m, sh.slot[4 * w]);
+            for (int w = 1; w < kWaves; w++) m = PROBS ? m + sh.slot[4 * w] : fmaxf(m, sh.slot[4 * w]);
             s = {m, 0.0f, 0.0f};
             for (int w = 0; w < kWaves; w++) {
                 Stats v = {sh.slot[4 * w], sh.slot[4 * w + 1], sh.slot[4 * w + 2]};
@@ -525,11 +530,11 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
         for (int i = 0; i < W; i++) {
             const float v = i >= from ? raw[i] : PROBS ? 0.0f : -INFINITY;
             if constexpr (PROBS) least = fminf(least, v);
-            add_value<PROBS>(v, s.m, s.S, s.T);
+            add_value<PROBS>(v, s);
         }
         s.S = reduce64(s.S, Add());
         s.T = reduce64(s.T, Add());
-        if constexpr (PROBS) least = reduce64(least, Min());
+        if constexpr (PROBS) s.m = reduce64(s.m, Add()), least = reduce64(least, Min());
         const Row<PROBS> row(s, least < 0.0f);
         if (a.entropy && lane == 0) a.entropy[r] = row.entropy();
         label.put(a, row, r, lane);
@@ -574,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
         const int from = (int)(job - r * p.parts) * p.chunks, to = min(from + p.chunks, n_chunks);
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
         const Label label(a, x, r, p.parts == 1 ? t : kScoreMaxLabels);
-        Stats s = {kLowest, 0.0f, 0.0f};
+        Stats s = {PROBS ? 0.0f : kLowest, 0.0f, 0.0f};
         float least = 0.0f, most = -INFINITY, second = -INFINITY;       // the best chunk, and the best value of the others
         int most_at = -1;
         // U chunks, T apart; CHECKED: some of them may lie behind the part's end or be the row's last one
@@ -619,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
                 for (int i = 0; i < W; i++) {
                     const float v = i >= twice ? raw[u][i] : PROBS ? 0.0f : -INFINITY;
                     if constexpr (PROBS) least = fminf(least, v);
-                    add_value<PROBS>(v, s.m, s.S, s.T);
+                    add_value<PROBS>(v, s);
                 }
             }
         };
@@ -683,7 +688,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
     for (size_t r = blockIdx.x; r < (size_t)a.rows; r += gridDim.x) {
         const X *x = static_cast<const X *>(a.x) + r * (size_t)a.ld;
         const Label label(a, x, r, t);
-        Stats s = {kLowest, 0.0f, 0.0f};
+        Stats s = {PROBS ? 0.0f : kLowest, 0.0f, 0.0f};
         float least = 0.0f;
         if (t < p.parts) {                          // (parts <= kThreads)
             const float4 v = p.stats[r * p.parts + t];
