@@ -136,7 +136,13 @@ int lcrc_posteriors_batch(lcrc_ctx *ctx, const float *mel, const int *off, int n
  * synchronised; the caller orders the launch against its own work through the
  * stream it passes.  Small launches (see lcrc_set_hidden_split) use scratch
  * buffers of the context: launches of ONE context must not overlap on the
- * device then -- issue them on one stream, or pin the fused kernel. */
+ * device then -- issue them on one stream, or pin the fused kernel.  So do
+ * launches of any size where the system is composed of several kernels
+ * (lcrc_create_system at other lengths than 31, LCRC at another geometry,
+ * models no fused kernel holds, lcrc_set_merger_fp8): a replayed graph counts
+ * as a launch.  That scratch memory is allocated by the first call of a size,
+ * which waits for the device, or ahead by lcrc_reserve; a call that would have
+ * to allocate while its stream is captured is refused (LCRC_E_UNSUPPORTED). */
 int lcrc_posteriors_device(lcrc_ctx *ctx, const float *d_mel, const int *d_off, int n_utts,
                            int n_rows, float *d_post, void *hip_stream);
 

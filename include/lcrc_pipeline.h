@@ -91,7 +91,8 @@ int lcrc_wave_to_posteriors(lcrc_ctx *ctx, const unsigned char *bytes, const lon
  * demand inside its first call (device staging, pinned features / posteriors / offsets; with max_wave_bytes > 0 -- after
  * lcrc_frontend_configure -- the byte buffers of the waveform entries too).  Optional: the entry points grow their buffers
  * themselves; page pinning is what that costs (~8 ms per 32 768 HU frames), and a caller with a set-up phase calls this
- * there.  Call it after lcrc_decoder_configure / lcrc_set_posterior_readback (they decide whether a pinned posterior
+ * there.  With it launches of that size can be captured into a graph (lcrc_posteriors_device).  Call it after
+ * lcrc_set_merger_fp8 and lcrc_decoder_configure / lcrc_set_posterior_readback (they decide whether a pinned posterior
  * buffer is needed at all).  Has no reference counterpart (the reference allocates per bunch, traps.cpp:63-101). */
 int lcrc_reserve(lcrc_ctx *ctx, int max_rows, int max_utts, long long max_wave_bytes);
 /* Zero-copy variant: lcrc_wave_stage_buffer returns the context's pinned byte buffer (valid until a later
@@ -277,7 +278,8 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *args, void *hip_s
  * other geometry than the shipped ones) with 8-bit operands: normalised inputs, weights and hidden activations in e4m3 with
  * a scale per 128, sums, biases, sigmoid, softmax and output transform as ever.  Opt-in: the operands keep 4 significant
  * bits, so posteriors lie around 1e-2 from those of the 32-bit nets (synthetic nets of 1500 hidden units: the largest
- * difference of a frame 1.4e-2 on average, 6.8e-2 at most).  The shipped LCRC shapes: LCRC_E_UNSUPPORTED. */
+ * difference of a frame 1.4e-2 on average, 6.8e-2 at most).  Launches of the context use its scratch memory then, at any size:
+ * they must not overlap (lcrc_posteriors_device).  The shipped LCRC shapes: LCRC_E_UNSUPPORTED. */
 int lcrc_posteriors_scored(lcrc_ctx *ctx, const float *mel, const int *off, int n_utts, float *post, const int *labels, int n_labels,
                            int k, float *logp, float *entropy, int *top_index, float *top_logp);
 int lcrc_set_merger_fp8(lcrc_ctx *ctx, int enabled);

@@ -492,6 +492,63 @@ void fill_output_transform(const lcrc_ctx *c, int *func, float (*oc)[4], float (
     *be = c->out_be;
 }
 
+// Scratch of the systems that are composed of several launches: features (d_feat), the merger's inputs (d_minp), the 8-bit
+// merger's operands (d_fp8).  It grows with the first call of a size (lcrc_reserve: ahead of it), but not while the call's stream
+// is captured; what a captured launch uses stays until the context's end, so that its graph can be replayed.
+bool traps_unfused(const lcrc_ctx *c)            // (the 8-bit merger reads its inputs from memory)
+{
+    return c->traps_unfused || c->fp8_merger || (c->system != SYS_1BT_DCT && c->bt_unfused);
+}
+int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s)
+{
+    bool captured = false;
+    if (s) {                                     // (HIP's default stream cannot be captured)
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s, &status) == hipSuccess) captured = status == hipStreamCaptureStatusActive;
+        else (void)hipGetLastError();
+    }
+    const size_t fp8 = c->fp8_merger ? merger_fp8_bytes(c, n_rows) : 0;
+    const bool more_rows = n_rows > c->cap_feat_rows, more_fp8 = fp8 > c->cap_fp8;
+    if (captured && (more_rows || more_fp8))
+        return fail(c, LCRC_E_UNSUPPORTED, "scratch memory for " + std::to_string(n_rows) + " frames cannot be allocated while the stream is captured: call lcrc_reserve first");
+    const auto drop = [&](void *p) {
+        if (p && c->scratch_in_graph) c->allocs.push_back(p);
+        else if (p) (void)hipFree(p);            // (waits for launches that still use it)
+    };
+    const auto get = [&](void **p, size_t bytes) {
+        if (dev_alloc(p, bytes) == hipSuccess) return true;
+        (void)hipGetLastError();
+        return false;
+    };
+    const std::string none = "cannot allocate scratch memory for " + std::to_string(n_rows) + " frames";
+    if (more_rows) {
+        const size_t cap = n_rows + n_rows / 4 + 64, Km = c->nets[2].n_inp;
+        drop(c->d_feat);
+        drop(c->d_minp);
+        c->d_feat = c->d_minp = nullptr;
+        c->cap_feat_rows = 0;
+        const size_t feat = c->system == SYS_1BT_DCT ? cap * Km
+                            : c->system == SYS_LCRC_GEN ? cap * 2 * (size_t)c->band_nets[0].n_inp
+                                                        : cap * (size_t)c->trap_bands * c->trap_len;
+        if (!get((void **)&c->d_feat, feat * sizeof(float))) return fail(c, LCRC_E_NOMEM, none);
+        if (c->system != SYS_1BT_DCT && !get((void **)&c->d_minp, cap * Km * sizeof(float))) {
+            (void)hipFree(c->d_feat);
+            c->d_feat = nullptr;
+            return fail(c, LCRC_E_NOMEM, none);
+        }
+        c->cap_feat_rows = cap;
+    }
+    if (more_fp8) {
+        drop(c->d_fp8);
+        c->d_fp8 = nullptr;
+        c->cap_fp8 = 0;
+        if (!get((void **)&c->d_fp8, fp8 + fp8 / 4)) return fail(c, LCRC_E_NOMEM, none);
+        c->cap_fp8 = fp8 + fp8 / 4;
+    }
+    if (captured) c->scratch_in_graph = true;
+    return LCRC_OK;
+}
+
 // 1BT_DCT: ONE launch (the merger's kernel computes its C0 / DCT input rows from the mel tile it stages).
 // 1BT / 3BT: features -> band nets (one launch, grid.y = band) -> merger, on the same stream.
 int launch_traps(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, int n_rows, float *d_post,
@@ -499,22 +556,11 @@ int launch_traps(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, 
 {
     if (n_rows <= 0) return LCRC_OK;
     const size_t Km = c->nets[2].n_inp;
-    const bool unfused = c->traps_unfused || c->fp8_merger;        // (the 8-bit merger reads its inputs from memory)
+    const bool unfused = traps_unfused(c);
     const bool fused_dct = c->system == SYS_1BT_DCT && !unfused;
-    const bool fused_bt = c->system != SYS_1BT_DCT && !unfused && !c->bt_unfused;
-    if (!fused_dct && !fused_bt && (size_t)n_rows > c->cap_feat_rows) {
-        const size_t cap = (size_t)n_rows + n_rows / 4 + 64;
-        if (c->d_feat) (void)hipFree(c->d_feat);
-        if (c->d_minp) (void)hipFree(c->d_minp);
-        c->d_feat = c->d_minp = nullptr;
-        c->cap_feat_rows = 0;
-        const size_t feat = c->system == SYS_1BT_DCT ? cap * Km
-                            : c->system == SYS_LCRC_GEN ? cap * 2 * (size_t)c->band_nets[0].n_inp
-                                                        : cap * (size_t)c->trap_bands * c->trap_len;
-        HIP_TRY(c, hipMalloc((void **)&c->d_feat, feat * sizeof(float)));
-        if (c->system != SYS_1BT_DCT) HIP_TRY(c, hipMalloc((void **)&c->d_minp, cap * Km * sizeof(float)));
-        c->cap_feat_rows = cap;
-    }
+    const bool fused_bt = c->system != SYS_1BT_DCT && !unfused;
+    if (unfused)
+        if (const int rc = ensure_traps_scratch(c, (size_t)n_rows, s)) return rc;
     TrapsFeatParams f;
     memset(&f, 0, sizeof f);
     f.mel = d_mel; f.off = d_off; f.n_utts = n_utts; f.n_rows = n_rows;

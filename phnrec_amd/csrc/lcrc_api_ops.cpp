@@ -99,21 +99,15 @@ namespace lcrc_impl {
 
 // ---- the merger of an unfused system with 8-bit operands (lcrc_set_merger_fp8) ----
 // inputs -> normalised, in 8 bits -> hidden layer (FEXP sigmoid), in 8 bits -> outputs in f32 -> softmax and output transform
+size_t merger_fp8_bytes(const lcrc_ctx *c, size_t n_rows)
+{
+    const NetDev &net = c->nets[2];
+    return (size_t)Q8Shape((int)n_rows, net.n_inp).bytes() + (size_t)Q8Shape((int)n_rows, net.n_hid).bytes() + n_rows * net.n_out * sizeof(float);
+}
 int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, hipStream_t s)
 {
     const NetDev &net = c->nets[2];
     const size_t x_bytes = (size_t)Q8Shape(n_rows, net.n_inp).bytes(), h_bytes = (size_t)Q8Shape(n_rows, net.n_hid).bytes();
-    const size_t need = x_bytes + h_bytes + (size_t)n_rows * net.n_out * sizeof(float);
-    if (need > c->cap_fp8) {
-        if (c->d_fp8) (void)hipFree(c->d_fp8);              // (waits for launches that still use it)
-        c->d_fp8 = nullptr;
-        c->cap_fp8 = 0;
-        if (dev_alloc((void **)&c->d_fp8, need + need / 4) != hipSuccess) {
-            (void)hipGetLastError();
-            return fail(c, LCRC_E_NOMEM, "cannot allocate the 8-bit merger's operands for " + std::to_string(n_rows) + " frames");
-        }
-        c->cap_fp8 = need + need / 4;
-    }
     unsigned char *x = c->d_fp8, *h = x + x_bytes;
     float *y = reinterpret_cast<float *>(h + h_bytes);
     const OpsTable *k;

@@ -349,6 +349,10 @@ int lcrc_reserve(lcrc_ctx *c, int max_rows, int max_utts, long long max_wave_byt
         rc = ensure_host_post(c);
         if (rc) return rc;
     }
+    if (c->system != SYS_LCRC && traps_unfused(c)) {
+        rc = ensure_traps_scratch(c, (size_t)std::max(max_rows, 1), c->stream);
+        if (rc) return rc;
+    }
     if (c->system == SYS_LCRC && !c->d_part && c->split_hint != 1 && c->arith == 0) ensure_split_scratch(c);
     if (c->dec_P > 0) {
         rc = ensure_labels(c, (size_t)std::max(max_rows, 1), (size_t)max_utts);

@@ -139,6 +139,7 @@ struct lcrc_ctx {
     bool fp8_merger = false;
     unsigned char *fp8_w1 = nullptr, *fp8_w2 = nullptr, *d_fp8 = nullptr;
     size_t cap_fp8 = 0;
+    bool scratch_in_graph = false;   // a captured launch uses d_feat / d_minp / d_fp8: they are kept when they grow
     // lcrc_posteriors_scored: labels, scores and scratch on the device, labels and scores in pinned host memory
     char *d_scores = nullptr, *h_scores = nullptr;
     size_t cap_scores = 0;
@@ -228,6 +229,9 @@ int run_host(lcrc_ctx *c, const float *mel, const int *off, int n_utts, int n, f
              const HostScores *scores = nullptr);
 int two_part_output(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, int n, float *post, bool *done);
 
+bool traps_unfused(const lcrc_ctx *c);
+int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s);
+
 // ---- lcrc_api_decoder.cpp ----
 int ensure_labels(lcrc_ctx *c, size_t n_rows, size_t n_utts);
 bool overlap_on(const lcrc_ctx *c);
@@ -245,6 +249,7 @@ int decode_after(lcrc_ctx *c, const int *d_off, const int *h_first, int n_utts, 
                  hipStream_t s, bool staged = false);
 
 // ---- lcrc_api_ops.cpp ----
+size_t merger_fp8_bytes(const lcrc_ctx *c, size_t n_rows);
 int merger_fp8(lcrc_ctx *c, const float *d_in, int n_rows, const MlpParams &m, hipStream_t s);
 
 }  // namespace lcrc_impl

@@ -14,9 +14,8 @@
 typedef struct { unsigned x, y, z; } dim3;
 typedef int hipError_t;
 
-atomic_int stub_inside, stub_loading, stub_beside_a_load, stub_calls, stub_launches, stub_frees, stub_capturing, stub_last_error;
+atomic_int stub_inside, stub_loading, stub_beside_a_load, stub_calls, stub_launches, stub_mallocs, stub_frees, stub_capturing, stub_last_error;
 int stub_load_us = 0;
-atomic_long stub_allocated;
 
 static int threads_of_this_process(void)
 {
@@ -68,7 +67,7 @@ static hipError_t get(void **p, size_t n)
 {
     enter();
     *p = calloc(1, n ? n : 1);
-    atomic_fetch_add(&stub_allocated, (long)n);
+    atomic_fetch_add(&stub_mallocs, 1);
     return leave();
 }
 static hipError_t put(void *p)
