@@ -250,7 +250,8 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
  * rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
  * n_in <= 2^23; W, x and y hold at most 2^26 tiles of 16 rows x 128 columns.
  * LCRC_ACT_SIGMOID: 1 / (1 + exp(-v)); LCRC_ACT_FSIGMOID: the same with the reference's fast exponential (fexp.h:14-21),
- * which its trained nets expect.  y overlaps no input. */
+ * which its trained nets expect (an exponential for |v| < 708; beyond it its integer wraps, here as there, and NaN is one of
+ * its arguments: the result is then no sigmoid and need not be NaN).  y overlaps no input. */
 enum { LCRC_ACT_NONE = 0, LCRC_ACT_SIGMOID = 1, LCRC_ACT_FSIGMOID = 2 };
 typedef struct lcrc_fp8_linear_args {
     const void *x;

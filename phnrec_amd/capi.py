@@ -24,7 +24,7 @@ SYMBOLS = [
     "lcrc_reset", "lcrc_push", "lcrc_delay",
     "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_debug_pinned_outside_rss", "lcrc_kernel_name",
     "lcrc_score_workspace", "lcrc_score", "lcrc_fp8_bytes", "lcrc_fp8_pack", "lcrc_fp8_unpack", "lcrc_fp8_linear_workspace", "lcrc_fp8_linear",
-    "lcrc_posteriors_scored", "lcrc_set_merger_fp8",
+    "lcrc_posteriors_scored", "lcrc_set_merger_fp8", "lcrc_debug_fp8_route",
 ]
 
 LCRC_OK, LCRC_E_ARG, LCRC_E_IO, LCRC_E_MODEL, LCRC_E_DEVICE, LCRC_E_NOMEM, LCRC_E_UNSUPPORTED = \
@@ -193,6 +193,7 @@ def load():
     L.lcrc_fp8_linear.argtypes = [C.c_int, C.POINTER(Fp8LinearArgs), vp]
     L.lcrc_posteriors_scored.argtypes = [vp, _f32p, vp, C.c_int, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp]
     L.lcrc_set_merger_fp8.argtypes = [vp, C.c_int]
+    L.lcrc_debug_fp8_route.argtypes = [C.c_int] * 4
     for name in ("lcrc_score_workspace", "lcrc_fp8_bytes", "lcrc_fp8_linear_workspace"):
         getattr(L, name).restype = C.c_size_t
     _lib = L

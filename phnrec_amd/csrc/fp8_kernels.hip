@@ -630,11 +630,10 @@ void split_launch(const Fp8ProductParams &p, const void *x, long long ldx, hipSt
     else if (p.n_out >= 16 * 512) split_launch<EXACT, X, 2, 1, 16>(p, x, ldx, stream);
     else split_launch<EXACT, X, 1, 1, 16>(p, x, ldx, stream);
 }
-bool sums_in_32_bits(const Fp8ProductParams &p) { return p.y_type == LCRC_T_F32 || p.y_type == LCRC_T_E4M3; }
 template <typename X>
 hipError_t split_by_sums(const Fp8ProductParams &p, const void *x, long long ldx, hipStream_t stream)
 {
-    if (sums_in_32_bits(p)) split_launch<true, X>(p, x, ldx, stream);
+    if (fp8_sums_in_32_bits(p.y_type)) split_launch<true, X>(p, x, ldx, stream);
     else split_launch<false, X>(p, x, ldx, stream);
     return hipGetLastError();
 }
@@ -644,12 +643,8 @@ void tile_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
     const long long across = ((long long)p.n_out + 16 * FW * WW - 1) / (16 * FW * WW), down = ((long long)p.rows + 16 * FX * WX - 1) / (16 * FX * WX);
     const long long blocks = (across * down + 7) / 8 * 8;
+    static_assert(WW * WX == 4, "fp8_route's tiles are 256 threads each");
     fp8_tile_kernel<EXACT, FW, FX, WW, WX, STAGES><<<(unsigned)blocks, 64 * WW * WX, 0, stream>>>(p, (int)across, (int)down);
-}
-// tiles of 16 FW WW outputs x 16 FX WX rows
-long long tiles(const Fp8ProductParams &p, int outputs, int rows)
-{
-    return (((long long)p.n_out + outputs - 1) / outputs) * (((long long)p.rows + rows - 1) / rows);
 }
 
 }  // namespace
@@ -685,19 +680,19 @@ hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream)
 
 hipError_t fp8_product_launch(const Fp8ProductParams &p, hipStream_t stream)
 {
-    // Which tiles (measured, us): large ones read least per product, but need two workgroups for every CU:
-    //   4096 x 8192 x 2048 bf16   256 x 128 (256 tiles) 86, 128 x 128 (512) 73, 128 x 64 100
-    //   777 x 1999 x 2309 f16     128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
-    // In short sums nothing is read often enough to count, and small tiles fill the card better:
-    //   8192 x 372 x 1500 in 8 bits  128 x 128 26.5, 128 x 64 25.3
-    const bool exact = sums_in_32_bits(p), longer = p.n_in > 512;
-    if (tiles(p, 128, 64) <= 128) return split_by_sums<unsigned char>(p, nullptr, 0, stream);
-    if (exact) {
-        if (longer && tiles(p, 128, 128) >= 512) tile_launch<true, 8, 2, 1, 4>(p, stream);
-        else tile_launch<true, 8, 1, 1, 4, 2>(p, stream);
-    } else if (longer && tiles(p, 256, 128) >= 512) tile_launch<false, 8, 4, 2, 2>(p, stream);
-    else if (longer && tiles(p, 128, 128) >= 512) tile_launch<false, 8, 2, 1, 4>(p, stream);
-    else tile_launch<false, 8, 1, 1, 4, 2>(p, stream);
+    const bool exact = fp8_sums_in_32_bits(p.y_type);
+    switch (fp8_route(p.rows, p.n_in, p.n_out, p.y_type)) {
+    case kFp8SharedSums: return split_by_sums<unsigned char>(p, nullptr, 0, stream);
+    case kFp8Tiles256x128: tile_launch<false, 8, 4, 2, 2>(p, stream); break;          // (not with sums in 32 bits)
+    case kFp8Tiles128x128:
+        if (exact) tile_launch<true, 8, 2, 1, 4>(p, stream);
+        else tile_launch<false, 8, 2, 1, 4>(p, stream);
+        break;
+    case kFp8Tiles128x64:
+        if (exact) tile_launch<true, 8, 1, 1, 4, 2>(p, stream);
+        else tile_launch<false, 8, 1, 1, 4, 2>(p, stream);
+        break;
+    }
     return hipGetLastError();
 }
 

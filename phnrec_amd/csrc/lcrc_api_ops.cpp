@@ -380,4 +380,9 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     return launched(call, k->fp8_product(p, s));
 }
 
+int lcrc_debug_fp8_route(int rows, int n_in, int n_out, int y_type)
+{
+    return fp8_route(rows, n_in, n_out, y_type) + (fp8_sums_in_32_bits(y_type) ? 4 : 0);
+}
+
 }  // extern "C"

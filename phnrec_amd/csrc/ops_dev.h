@@ -73,6 +73,26 @@ struct Q8Shape {
     __host__ __device__ long long bytes() const { return scales_at() + rt * kb4 * (kQRows * 4); }
 };
 
+// Which kernel makes a product (measured, us): large tiles of outputs x rows read least per product, but need two workgroups for
+// every CU:
+//   4096 x 8192 x 2048 bf16   256 x 128 (256 tiles) 86, 128 x 128 (512) 73, 128 x 64 100
+//   777 x 1999 x 2309 f16     128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
+// In short sums nothing is read often enough to count, and small tiles fill the card better:
+//   8192 x 372 x 1500 in 8 bits  128 x 128 26.5, 128 x 64 25.3
+enum Fp8Route { kFp8SharedSums = 0, kFp8Tiles128x64 = 1, kFp8Tiles128x128 = 2, kFp8Tiles256x128 = 3 };
+inline long long fp8_tiles(int rows, int n_out, int tile_outputs, int tile_rows)
+{
+    return (((long long)n_out + tile_outputs - 1) / tile_outputs) * (((long long)rows + tile_rows - 1) / tile_rows);
+}
+inline bool fp8_sums_in_32_bits(int y_type) { return y_type == LCRC_T_F32 || y_type == LCRC_T_E4M3; }
+inline Fp8Route fp8_route(int rows, int n_in, int n_out, int y_type)
+{
+    if (fp8_tiles(rows, n_out, 128, 64) <= 128) return kFp8SharedSums;
+    if (n_in <= 512) return kFp8Tiles128x64;
+    if (!fp8_sums_in_32_bits(y_type) && fp8_tiles(rows, n_out, 256, 128) >= 512) return kFp8Tiles256x128;
+    return fp8_tiles(rows, n_out, 128, 128) >= 512 ? kFp8Tiles128x128 : kFp8Tiles128x64;
+}
+
 struct Fp8PackParams {
     const void *src;
     const unsigned char *scales;   // type e4m3: [rows][ceil(cols / 128)], biased by 127

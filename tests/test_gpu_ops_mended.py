@@ -58,7 +58,8 @@ def _other_system(tmp_path, capi, system, nb=15, n_out=48, hidden=200):
     if system == "LCRC":                                     # a geometry of its own: trajectories of 21 frames
         nets = modelgen.write_model_dir(d, nb, hidden, n_out, seed=hidden, trap_len=21)
         return capi.Lcrc(d, nb, trap_len=21), nets
-    return capi.Lcrc(d, nb, system=system), modelgen.write_traps_dir(d, system, nb, hidden, n_out, seed=hidden, coefs=6)
+    nets = modelgen.write_traps_dir(d, system, nb, hidden, n_out, seed=hidden, coefs=6)
+    return capi.Lcrc(d, nb, system=system), nets
 
 
 @pytest.mark.parametrize("system", ["1BT_DCT", "1BT", "3BT", "LCRC"])

@@ -42,3 +42,12 @@ def test_the_command_line_does_not_load_it(tmp_path):
                         os.path.join(GOLD, "test.raw"), "-t", "par", "-o", str(tmp_path / "o")], env=dict(os.environ, LD_DEBUG="files"),
                        capture_output=True, text=True)
     assert p.returncode == 0 and "libphnrec_lcrc.so" in p.stderr and "lcrc_ops" not in p.stderr
+
+
+def test_the_products_test_sizes_reach_every_kernel():
+    """(a change of lcrc_fp8_linear's choice must not leave one of its kernels untested)"""
+    from tests import test_gpu_fp8_tiles as tiles
+    tiles.test_the_sizes_reach_every_kernel(capi)
+    for size in tiles.SIZES:
+        for y in ("bf16", "f32"):
+            tiles._route(capi, size, y)
