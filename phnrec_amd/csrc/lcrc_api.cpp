@@ -630,6 +630,7 @@ int launch_traps(lcrc_ctx *c, const float *d_mel, const int *d_off, int n_utts, 
     if (c->fp8_merger) {
         const int rc = merger_fp8(c, merger_in, n_rows, m, s);
         if (rc) return rc;
+        c->mlp_variant = "fp8";
     } else HIP_TRY(c, mlp_launch(m, s, &c->mlp_variant));
     if (c->timing) { HIP_TRY(c, hipEventRecord(c->ev1, s)); c->timed = true; }
     return LCRC_OK;

@@ -57,8 +57,12 @@ def _other_system(tmp_path, capi, system, nb=15, n_out=48, hidden=200):
     d = str(tmp_path / "m")
     if system == "LCRC":                                     # a geometry of its own: trajectories of 21 frames
         nets = modelgen.write_model_dir(d, nb, hidden, n_out, seed=hidden, trap_len=21)
+    else:
+        nets = modelgen.write_traps_dir(d, system, nb, hidden, n_out, seed=hidden, coefs=6)
+    for i, name in enumerate(sorted(n for n in nets if n.startswith("band"))):
+        nets[name] = _few_terms("%s/weights/%s.nbin" % (d, name), nets[name], i)
+    if system == "LCRC":
         return capi.Lcrc(d, nb, trap_len=21), nets
-    nets = modelgen.write_traps_dir(d, system, nb, hidden, n_out, seed=hidden, coefs=6)
     return capi.Lcrc(d, nb, system=system), nets
 
 
@@ -102,3 +106,107 @@ def test_a_graph_of_the_8_bit_merger_and_larger_launches_behind_it(capi, tmp_pat
             assert launch(rows, post, _stream()) == 0
             torch.cuda.synchronize()
             assert np.array_equal(got, post.cpu().numpy()) and all((t == 7.0).all() for t in filler)
+
+
+def _few_terms(path, net, seed):
+    """a band net whose sums have one term each, weights that are powers of two and inputs as they come: what 32 bits compute of it
+    is known to a few roundings"""
+    from phnrec_amd import modelgen
+    rng = np.random.default_rng(seed)
+    net = {k: np.zeros_like(v) for k, v in net.items()}
+    hid, n_in = net["w1"].shape
+    out = net["w2"].shape[0]
+    net["dev"] += 1
+    net["w1"][np.arange(hid), rng.permutation(np.arange(hid) % n_in)] = rng.choice([-1, 1], hid) * 2.0 ** -rng.integers(3, 5, hid)
+    net["w2"][np.arange(out), rng.permutation(np.arange(out) % hid)] = rng.choice([-1, 1], out) * 2.0 ** rng.integers(1, 3, out)
+    modelgen.write_nbin(path, net)
+    return net
+
+
+def _net(net, x, dx, terms, hold):
+    """the reference's net (Normalize, two layers, FEXP sigmoid) on x in 64 bits, x being off by at most dx: outputs before the
+    softmax and how far a computation in 32 bits may be from them.  Sums of so many terms; FEXP and the sigmoid are monotonous, so
+    the ends bound them.  hold: with operands in 8 bits, sums in 32"""
+    from tests.test_gpu_ops_context import _fexp, _held
+    mean, dev, w1, b1, w2, b2 = (np.asarray(net[n], np.float64) for n in ("mean", "dev", "w1", "b1", "w2", "b2"))
+    v = (x - mean) * dev
+    dv = dx * np.abs(dev) + 2 * EPS * (np.abs(x) + np.abs(mean)) * np.abs(dev) * (mean != 0)
+    if hold:
+        v, dv = _held(v, dv)
+        w1, w2 = ref.held(w1)[0], ref.held(w2)[0]
+    z = v @ w1.T + b1
+    dz = dv @ np.abs(w1).T + (terms or v.shape[1] + 2) * EPS * ((np.abs(v) + dv) @ np.abs(w1).T + np.abs(b1))
+    h = 1 / (1 + _fexp(-z))
+    dh = np.maximum(np.abs(1 / (1 + _fexp(-(z + dz))) - h), np.abs(1 / (1 + _fexp(-(z - dz))) - h)) + 4 * EPS
+    if hold:
+        h, dh = _held(h, dh)
+    y = h @ w2.T + b2
+    return y, dh @ np.abs(w2).T + (terms or w2.shape[1] + 2) * EPS * ((h + dh) @ np.abs(w2).T + np.abs(b2))
+
+
+def _softmax(y, dy):
+    """posteriors with FEXP, and by what factor (minus 1) each may be off: FEXP rises by 1 / ln 2 of its argument at most, in steps of
+    2^-20; a sum of n terms, a quotient"""
+    from tests.test_gpu_ops_context import _fexp
+    e = _fexp(y - y.max(1, keepdims=True))
+    return e / e.sum(1, keepdims=True), np.expm1(2 * 1.45 * dy.max(1, keepdims=True)) + 2 * 2.0 ** -20 + (y.shape[1] + 4) * EPS
+
+
+def _merger_inputs(system, nets, mel, length):
+    """the merger's input rows of 1BT, 3BT and LCRC, and how far 32 bits may be from them"""
+    from phnrec_amd import modelgen
+    rows, nb = mel.shape
+    back = length - 1 - (length - 1) // 2
+    at = np.clip(np.arange(rows)[:, None] - back + np.arange(length)[None], 0, rows - 1)
+    t = mel.astype(np.float64)[at].transpose(0, 2, 1)                             # [rows][bands][length]
+    cols, errs = [], []
+    if system == "LCRC":
+        half = (length - 1) // 2 + 1
+        basis = np.stack([np.ones(half)] + [np.cos(np.pi * v / half * (np.arange(half) + 0.5)) for v in range(1, 11)])
+        for i, win in enumerate(modelgen.half_windows(half)):
+            win = np.array([float("%.7e" % v) for v in win], np.float32).astype(np.float64)
+            part = (t[:, :, :half] if i == 0 else t[:, :, half - 1:]) * win
+            f = (np.sqrt(2 / half) * (part @ basis.T)).reshape(rows, -1)
+            # (window, basis value -- off by a rounding and by its argument's, 2^-22 --, product, half sums, scale)
+            df = (half + 12) * EPS * (np.sqrt(2 / half) * np.abs(part).sum(2)).repeat(11, 1).reshape(rows, -1)
+            p, rel = _softmax(*_net(nets["band%d" % i], f, df, 2, False))
+            cols.append(np.log(p))
+            errs.append(np.log1p(rel) + 4 * EPS * np.abs(np.log(p)))
+    else:
+        for b in range(nb - 2 if system == "3BT" else nb):
+            p, rel = _softmax(*_net(nets["band%d" % b], t[:, b], np.zeros_like(t[:, b]), 2, False))
+            cols.append(-np.log(p))
+            errs.append(np.log1p(rel) + 4 * EPS * np.abs(np.log(p)))
+    return np.concatenate(cols, 1), np.concatenate([np.broadcast_to(e, c.shape) for e, c in zip(errs, cols)], 1)
+
+
+@pytest.mark.parametrize("rows", [1, 70, 401])
+@pytest.mark.parametrize("system", ["1BT", "3BT", "LCRC"])
+def test_merger_in_8_bits_behind_band_nets(capi, tmp_path, system, rows):
+    """the whole chain in 64 bits, its bounds step by step (a held value moves by the steps that its error crosses); the f32 merger
+    against the same chain without 8 bits, and the oracle's merger inputs against these"""
+    from contextlib import closing
+    from oracle import binding
+    from phnrec_amd import modelgen
+    ctx, nets = _other_system(tmp_path, capi, system)
+    length = 21 if system == "LCRC" else 31
+    mel = modelgen.synth_mel(rows, 15, seed=rows).astype(np.float32).reshape(rows, 15)
+    off = np.array([0, rows], np.int32)
+    with closing(ctx):
+        full = ctx.posteriors_batch(mel, off)
+        ctx.set_merger_fp8(True)
+        got = ctx.posteriors_batch(mel, off)
+        s = ctx.posteriors_scored(mel, off, None, 3)
+        assert np.array_equal(s["post"], got)
+        ctx.set_merger_fp8(False)
+        assert np.array_equal(ctx.posteriors_batch(mel, off), full)
+    g, dg = _merger_inputs(system, nets, mel, length)
+    theirs = np.zeros(g.shape, np.float32)
+    orc = binding.TrapsOracle(str(tmp_path / "m"), system, 15, trap_len=length)
+    orc.L.orc_traps_posteriors_batch(orc.h, mel, off, 1, np.zeros(full.shape, np.float32), theirs.ctypes.data)
+    assert (np.abs(theirs - g) <= dg).all()
+    for have, hold in ((full, False), (got, True)):
+        p, rel = _softmax(*_net(nets["merger"], g, dg, 0, hold))
+        assert rows == 1 or np.median(rel) < 0.01      # (the bounds say something)
+        assert (np.abs(have - p) <= p * rel + full.shape[1] * EPS).all(), (hold, np.abs(have - p).max(), rel.max())
+    assert not np.array_equal(got, full)
