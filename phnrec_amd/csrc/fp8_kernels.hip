@@ -223,10 +223,11 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
 // The 8-bit matrix instructions multiply exactly, but inside a group of eight products (eight bytes of a lane that follow one
 // another) they cut every product off 13 bits below the group's largest one before they add (measured, for the scaled and the
 // plain form alike: 2^16 + 3 * 2^3 comes out whole, of 2^16 + 3 * 7 the sevens are gone); the groups' sums are added in 32
-// bits.  That is up to 7 * 2^-13 of the products' absolute sum, 1.4e-5 relative on normal values: nothing beside a result
-// that is rounded to 16 bits (2^-8, 2^-11), too much for one in 32 bits -- and for one in 8, whose rounding turns 1.4e-5 into
-// a whole step, 2^-3, wherever it lies that near to a border: a net with hidden values in 8 bits and results in f16 was off by
-// 5.5e-4 of its results where sums in 32 bits leave 2.1e-4.  So products with such results turn their operands into bf16 --
+// bits.  That is up to 7 * 2^-13 = 0.22 * 2^-8 of the products' absolute sum, 1.4e-5 relative on normal values: beside the
+// rounding of a result to bf16, 2^-8, a fifth at the very most, in 3 of 1000 results the other neighbour.  It is more than f16's
+// rounding, 2^-11; too much for a result in 32 bits; and for one in 8, whose rounding turns 1.4e-5 into a whole step, 2^-3,
+// wherever it lies that near to a border: a net with hidden values in 8 bits was off by 5.5e-4 of its results where sums in 32
+// bits leave 2.1e-4.  So products with results in anything but bf16 turn their operands into bf16 --
 // exact: 4 significant bits, the block's scale goes into bf16's exponent (v_cvt_scalef32_pk_bf16_fp8; below 2^-126 it loses
 // bits) -- and use the bf16 instruction, whose sums are f32 throughout: half the rate.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));

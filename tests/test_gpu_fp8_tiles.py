@@ -15,7 +15,7 @@ EXACT = 4                                                    # of a route: sums 
 # rows, n_in, n_out: the route of results in bf16 and of those that come from sums in 32 bits
 SIZES = {(33, 700, 300): (0, 0), (1031, 300, 1999): (1, 1), (777, 1030, 2309): (1, 1), (2100, 1030, 4100): (2, 2), (4100, 1030, 8200): (3, 2),
          (9001, 129, 140): (1, 1), (513, 2049, 17000): (2, 2)}
-IN_32_BITS = ("f32", "e4m3")
+IN_32_BITS = ("f32", "f16", "e4m3")
 
 
 @pytest.fixture(scope="module")
@@ -51,7 +51,7 @@ def _whole_numbers(rng, rows, n_in, n_out):
     return x, w, rng.integers(-50, 51, n_out).astype(np.float64)
 
 
-@pytest.mark.parametrize("y_type", ["f32", "e4m3", "bf16"])
+@pytest.mark.parametrize("y_type", ["f32", "f16", "e4m3", "bf16"])
 @pytest.mark.parametrize("size", list(SIZES))
 def test_products_of_whole_numbers(capi, size, y_type):
     rows, n_in, n_out = size
@@ -70,6 +70,8 @@ def test_products_of_whole_numbers(capi, size, y_type):
     want = _product(x, w) + b
     if y_type == "f32":
         assert np.array_equal(got, want)
+    elif y_type == "f16":
+        assert np.array_equal(got, want.astype(np.float16).astype(np.float64))
     elif y_type == "e4m3":
         assert np.array_equal(got, ref.held(want)[0])
     else:
@@ -80,7 +82,7 @@ def test_products_of_whole_numbers(capi, size, y_type):
 
 
 @pytest.mark.parametrize("act", ["none", "sigmoid", "fsigmoid"])
-@pytest.mark.parametrize("x_type,y_type", [("bf16", "bf16"), ("f16", "f32"), ("f32", "e4m3"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("x_type,y_type", [("bf16", "bf16"), ("f16", "f32"), ("f32", "e4m3"), ("e4m3", "bf16"), ("f16", "f16")])
 @pytest.mark.parametrize("size", [s for s in SIZES if s[0] * s[2] < 2e7])
 @pytest.mark.filterwarnings("ignore::RuntimeWarning")
 def test_products_against_64_bits(capi, size, x_type, y_type, act):
@@ -128,5 +130,5 @@ def test_products_against_64_bits(capi, size, x_type, y_type, act):
 
 
 def test_the_sizes_reach_every_kernel(capi):
-    seen = {capi.load().lcrc_debug_fp8_route(*size, capi.TYPES[y]) for size in SIZES for y in ("bf16", "f32")}
+    seen = {capi.load().lcrc_debug_fp8_route(*size, capi.TYPES[y]) for size in SIZES for y in ("bf16", "f16", "f32")}
     assert seen == {0, 1, 2, 3, 4, 5, 6}
