@@ -249,7 +249,8 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
  * 7 * 2^-13 of sum |x w|, a fifth of a rounding to bf16.)  x is a matrix in that form (LCRC_T_E4M3, ldx ignored) or is put into
  * it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32, f16 or bf16
  * rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
- * n_in <= 2^23; W, x and y hold at most 2^26 tiles of 16 rows x 128 columns.
+ * n_in <= 2^23; W, x and y hold fewer than 2^26 tiles of 16 rows x 128 columns (so does a matrix that is packed or unpacked),
+ * y fewer than 2^24 - 7 of 64 rows x 128 columns, what is begun counting as a whole one.
  * LCRC_ACT_SIGMOID: 1 / (1 + exp(-v)); LCRC_ACT_FSIGMOID: the same with the reference's fast exponential (fexp.h:14-21),
  * which its trained nets expect (an exponential for |v| < 708; beyond it its integer wraps, here as there, and NaN is one of
  * its arguments: the result is then no sigmoid and need not be NaN).  y overlaps no input. */

@@ -89,7 +89,7 @@ int check_held(const char *call, const void *p, int rows, int cols)
 {
     if (!p || !aligned(p, 16)) return bad(call, "an 8-bit matrix must be aligned to 16 bytes");
     const Q8Shape s(rows, cols);
-    if (s.rt * s.kb > kQMaxTiles) return bad(call, "an 8-bit matrix of more than 2^26 tiles of 16 x 128");
+    if (s.rt * s.kb >= kQMaxTiles) return bad(call, "an 8-bit matrix of 2^26 tiles of 16 x 128 or more");
     return LCRC_OK;
 }
 
@@ -359,7 +359,12 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     } else if (const int rc = check_rows(call, a->y, a->y_type, a->n_out, a->ldy)) return rc;
     if (const int rc = check_held(call, a->w, a->n_out, a->n_in)) return rc;
     const Q8Shape sx(a->rows, a->n_in), sy(a->rows, a->n_out);
-    if (sx.rt * sx.kb > kQMaxTiles || sy.rt * sy.kb > kQMaxTiles) return bad(call, "x or y of more than 2^26 tiles of 16 x 128");
+    if (sx.rt * sx.kb >= kQMaxTiles || sy.rt * sy.kb >= kQMaxTiles) return bad(call, "x or y of 2^26 tiles of 16 x 128 or more");
+    // (a last tile of outputs or rows counts as a whole one)
+    const Fp8Route route = fp8_route(a->rows, a->n_in, a->n_out, a->y_type);
+    if (route != kFp8SharedSums &&
+        fp8_tiles(a->rows, a->n_out, route == kFp8Tiles256x128 ? 256 : 128, route == kFp8Tiles128x64 ? 64 : 128) + 7 >= (1ll << 32) / 256)
+        return bad(call, "more rows and outputs than a grid has threads for");
     if (!aligned(a->bias, 4)) return bad(call, "bias must be aligned to 4 bytes");
     const size_t need = lcrc_fp8_linear_workspace(a->rows, a->n_in, a->x_type);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)))

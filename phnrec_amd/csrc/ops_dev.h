@@ -116,7 +116,7 @@ struct Fp8ProductParams {
     long long ldy;
 };
 constexpr int kQFewOut = 1 << 25;     // outputs of a product that converts its rows itself
-constexpr long long kQMaxTiles = 1ll << 26;      // of a matrix in the 8-bit form, of x and of y (a grid holds 2^32 threads)
+constexpr long long kQMaxTiles = 1ll << 26;      // a matrix in the 8-bit form, x and y have fewer: 64 threads each, and a grid has fewer than 2^32
 constexpr int kQMaxIn = 1 << 23;      // columns of the operands of a product: their tiles' offsets stay within 32 bits
 
 // ---- the kernels' object ----------------------------------------------------------------------------------------------

@@ -51,3 +51,35 @@ def test_the_products_test_sizes_reach_every_kernel():
     for size in tiles.SIZES:
         for y in ("bf16", "f32"):
             tiles._route(capi, size, y)
+
+
+P = 1 << 20
+
+
+def test_sizes_beyond_a_grid_are_refused():
+    """a grid has fewer than 2^32 threads: 64 to a tile of 16 x 128, 256 to 64 x 128 results (nothing reaches a GPU here: the arguments
+    are refused before one is asked for)"""
+    import pytest
+
+    def code(fn, *a, **k):
+        with pytest.raises(capi.LcrcError) as e:
+            fn(*a, **k)
+        return e.value.code
+
+    over, under = capi.LCRC_E_ARG, capi.LCRC_E_DEVICE         # (no GPU here: what passes the checks fails for that)
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("GPU present")
+    assert code(capi.fp8_pack, P, capi.T_F32, 1 << 30, 128, 128, P) == over
+    assert code(capi.fp8_pack, P, capi.T_F32, (1 << 30) - 16, 128, 128, P) == under
+    assert code(capi.fp8_unpack, P, 1 << 30, 128, P, capi.T_F32, 128) == over
+    assert code(capi.fp8_unpack, P, 1 << 30, 1, P, capi.T_F32, 128) == over
+    assert code(capi.fp8_unpack, P, (1 << 30) - 16, 1, P, capi.T_F32, 128) == under
+
+    def linear(rows, n_in, n_out):
+        a = capi.Fp8LinearArgs(x=P, x_type=capi.T_E4M3, rows=rows, n_in=n_in, n_out=n_out, ldx=0, w=P, act=0, y=P, y_type=capi.T_BF16, ldy=n_out)
+        return code(capi.fp8_linear, a)
+
+    assert linear(1 << 30, 128, 128) == over and linear((1 << 30) - 1024, 128, 128) == under
+    assert linear(129, 1, 128 * 7400000) == over              # 9 x 7.4 million tiles of 16 x 128, but 3 x 7.4 million of 64 x 128
+    assert linear(129, 1, 128 * 5500000) == under
