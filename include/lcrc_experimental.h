@@ -57,6 +57,10 @@ int lcrc_debug_fail_launch(int nth);
  * of its own instead of the process's pages leaves all of them out (phnrec's PHNREC_STATS adds them to max_rss_mb). */
 long long lcrc_debug_pinned_outside_rss(void);
 
+/* The largest number of workgroups of an lcrc_score launch from now on, 1 .. 2^22 (the default); returns what it was.  With few of
+ * them each takes many rows one after another, as it does of matrices with more rows than a grid has places.  For tests; not while
+ * another thread calls lcrc_score. */
+int lcrc_debug_score_blocks(int most);
 /* Which kernel lcrc_fp8_linear makes a product of this size with (for tests that have to reach each of them): 0 sums shared out
  * over a workgroup's waves; tiles of 1: 128 x 64, 2: 128 x 128, 3: 256 x 128 outputs x rows; + 4 where the sums are kept in 32
  * bits throughout. */

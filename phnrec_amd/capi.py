@@ -24,7 +24,7 @@ SYMBOLS = [
     "lcrc_reset", "lcrc_push", "lcrc_delay",
     "lcrc_last_kernel_ms", "lcrc_set_timing", "lcrc_set_wait_mode", "lcrc_set_kernel_done_callback", "lcrc_set_tile_frames", "lcrc_set_hidden_split", "lcrc_set_arithmetic", "lcrc_debug_fail_alloc", "lcrc_debug_fail_launch", "lcrc_debug_pinned_outside_rss", "lcrc_kernel_name",
     "lcrc_score_workspace", "lcrc_score", "lcrc_fp8_bytes", "lcrc_fp8_pack", "lcrc_fp8_unpack", "lcrc_fp8_linear_workspace", "lcrc_fp8_linear",
-    "lcrc_posteriors_scored", "lcrc_set_merger_fp8", "lcrc_debug_fp8_route",
+    "lcrc_posteriors_scored", "lcrc_set_merger_fp8", "lcrc_debug_fp8_route", "lcrc_debug_score_blocks",
 ]
 
 LCRC_OK, LCRC_E_ARG, LCRC_E_IO, LCRC_E_MODEL, LCRC_E_DEVICE, LCRC_E_NOMEM, LCRC_E_UNSUPPORTED = \

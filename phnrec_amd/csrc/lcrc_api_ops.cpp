@@ -385,6 +385,14 @@ int lcrc_fp8_linear(int device_id, const lcrc_fp8_linear_args *a, void *hip_stre
     return launched(call, k->fp8_product(p, s));
 }
 
+int lcrc_debug_score_blocks(int most)
+{
+    const OpsTable *k;
+    if (most < 1 || most > 1 << 22) return fail(nullptr, LCRC_E_ARG, "lcrc_debug_score_blocks: 1 .. 2^22");
+    if (const int rc = kernels(nullptr, &k)) return rc;
+    return k->score_most_blocks(most);
+}
+
 int lcrc_debug_fp8_route(int rows, int n_in, int n_out, int y_type)
 {
     return fp8_route(rows, n_in, n_out, y_type) + (fp8_sums_in_32_bits(y_type) ? 4 : 0);

@@ -129,7 +129,9 @@ struct OpsTable {
     // up to kQRows rows of f32, f16 or bf16: converted by the product itself (p.x is not read)
     hipError_t (*fp8_few_rows)(const Fp8ProductParams &p, const void *x, int x_type, long long ldx, hipStream_t stream);
     hipError_t (*softmax_rows)(const SoftmaxRowsParams &p, hipStream_t stream);
+    int (*score_most_blocks)(int most);          // of a launch from now on -> what it was
 };
+int score_most_blocks(int most);
 hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream);
 hipError_t fp8_pack_launch(const Fp8PackParams &p, hipStream_t stream);
 hipError_t fp8_unpack_launch(const Fp8UnpackParams &p, hipStream_t stream);

@@ -728,12 +728,12 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
 }
 
 // ---- which kernel, on what grid ----
-constexpr int kMaxBlocks = 1 << 22;      // beyond it the workgroups take several rows each
+int most_blocks = 1 << 22;               // beyond it the workgroups take several rows each (lcrc_debug_score_blocks)
 
 template <typename X, bool PROBS, int W, int J>
 void launch_short(const lcrc_score_args &a, int k, hipStream_t stream)
 {
-    const int blocks = (int)std::min<long long>(((long long)a.rows + kThreads / 8 - 1) / (kThreads / 8), kMaxBlocks);
+    const int blocks = (int)std::min<long long>(((long long)a.rows + kThreads / 8 - 1) / (kThreads / 8), most_blocks);
     if (k == 0) score_short_kernel<X, PROBS, W, J, 0><<<blocks, kThreads, 0, stream>>>(a);
     else if (k == 1) score_short_kernel<X, PROBS, W, J, 1><<<blocks, kThreads, 0, stream>>>(a);
     else if (k <= 3) score_short_kernel<X, PROBS, W, J, 3><<<blocks, kThreads, 0, stream>>>(a);
@@ -754,7 +754,7 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
     else if (k <= 8 && chunks <= 48) launch_short<X, PROBS, W, 6>(a, k, stream);
     else if (k <= 8 && chunks <= 64) launch_short<X, PROBS, W, 8>(a, k, stream);
     else if (chunks <= kScoreWaveChunks) {
-        const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, kMaxBlocks);
+        const int blocks = (int)std::min<long long>(((long long)a.rows + 3) / 4, most_blocks);
         const Part p = {1, chunks, nullptr, nullptr};
         if (chunks <= kScoreHeldChunks) score_wave_kernel<X, PROBS><<<blocks, kThreads, 0, stream>>>(a);
         else score_long_kernel<X, PROBS, 64><<<blocks, kThreads, 0, stream>>>(a, p);
@@ -763,16 +763,23 @@ hipError_t launch(const lcrc_score_args &a, hipStream_t stream)
         const size_t jobs = (size_t)a.rows * cut.parts;
         float4 *const stats = static_cast<float4 *>(a.workspace);
         const Part p = {cut.parts, cut.chunks, stats, reinterpret_cast<u64 *>(stats + (cut.parts > 1 ? jobs : 0))};
-        score_long_kernel<X, PROBS, kThreads><<<(int)std::min<size_t>(jobs, kMaxBlocks), kThreads, 0, stream>>>(a, p);
+        score_long_kernel<X, PROBS, kThreads><<<(int)std::min<size_t>(jobs, (size_t)most_blocks), kThreads, 0, stream>>>(a, p);
         if (p.parts > 1) {
             if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-            score_join_kernel<X, PROBS><<<std::min(a.rows, kMaxBlocks), kThreads, 0, stream>>>(a, p);
+            score_join_kernel<X, PROBS><<<std::min(a.rows, most_blocks), kThreads, 0, stream>>>(a, p);
         }
     }
     return hipGetLastError();
 }
 
 }  // namespace
+
+int score_most_blocks(int most)
+{
+    const int before = most_blocks;
+    most_blocks = most;
+    return before;
+}
 
 hipError_t score_launch(const lcrc_score_args &a, hipStream_t stream)
 {

@@ -210,3 +210,65 @@ def test_merger_in_8_bits_behind_band_nets(capi, tmp_path, system, rows):
         assert rows == 1 or np.median(rel) < 0.01      # (the bounds say something)
         assert (np.abs(have - p) <= p * rel + full.shape[1] * EPS).all(), (hold, np.abs(have - p).max(), rel.max())
     assert not np.array_equal(got, full)
+
+
+@pytest.mark.parametrize("form", ["logits", "probs"])
+@pytest.mark.parametrize("cols,k,type", [(9, 3, "f16"), (138, 5, "f32"), (300, 8, "bf16"), (138, 20, "f32"), (400, 64, "f16"), (3000, 16, "f16"),
+                                         (3000, 5, "f32"), (20000, 64, "bf16"), (70000, 7, "f32"), (140000, 33, "f16")])
+@pytest.mark.parametrize("blocks", [1, 3])
+def test_rows_that_a_workgroup_takes_one_after_another(capi, cols, k, type, form, blocks):
+    """few workgroups over many rows: every row as in a grid with a place for each, bit for bit, whatever the row in front of it was --
+    ties, more candidates than fit, no class left, no number"""
+    rows = 150 if cols < 1000 else 40 if cols < 50000 else 5
+    rng = np.random.default_rng(cols + k)
+    a = rng.standard_normal((rows, cols)) * 3
+    a[1::7] = np.round(a[1::7])                              # ties
+    a[2::7] = 1.0                                            # nothing but ties
+    a[3::7] = -np.inf
+    a[4::7, cols // 2] = np.nan
+    a[5::7] = np.arange(cols) / cols
+    if form == "probs":
+        a = np.exp(np.where(np.isnan(a), 0, a)) * np.where(np.isnan(a), np.nan, 1)
+        a[6::7, 0] = -1
+    x, exact = _strided(a, type, 3)
+    labels = rng.integers(-1, cols, (rows, 9))
+    L = capi.load()
+    want = Scored(capi, x, type, form, labels, k, cols).run().get()
+    before = L.lcrc_debug_score_blocks(blocks)
+    assert before == 1 << 22
+    try:
+        got = Scored(capi, x, type, form, labels, k, cols).run().get()
+    finally:
+        assert L.lcrc_debug_score_blocks(before) == blocks
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w, equal_nan=True)
+    w_logp, w_ent, w_ti, w_tl = ref.score(exact, labels, k, form)
+    lp, en = ref.score_tolerance(np.where(np.isfinite(exact) | np.isneginf(exact), exact, 0.5) if form == "logits" else np.abs(np.nan_to_num(exact)), form)
+    assert np.array_equal(got[2], w_ti)
+    _close(got[0], w_logp, lp[:, None])
+    _close(got[1], w_ent, en)
+    assert L.lcrc_debug_score_blocks(0) == capi.LCRC_E_ARG
+
+
+def test_more_short_rows_than_a_grid_has_lanes_for(capi):
+    """beyond 2^27 rows a group of 8 lanes takes a second one"""
+    base = 1 << 12
+    rows = (1 << 27) + base
+    rng = np.random.default_rng(2)
+    some = torch.from_numpy(np.round(rng.standard_normal((base, 2)) * 2).astype(np.float16)).cuda()
+    x = some.repeat(rows // base, 1)
+    x[-1, 0] = float("nan")
+    ti = torch.full((rows + 8, 2), 7, dtype=torch.int32, device="cuda")
+    ent = torch.full((rows + 8,), 7.0, device="cuda")
+    capi.score(capi.ScoreArgs(x=x.data_ptr(), type=capi.T_F16, form=0, rows=rows, cols=2, ld=2, k=2, entropy=ent.data_ptr(),
+                              top_index=ti.data_ptr()), stream=_stream())
+    torch.cuda.synchronize()
+    assert (ti[rows:] == 7).all() and (ent[rows:] == 7).all()
+    assert (ti[rows - 1] == -1).all() and torch.isnan(ent[rows - 1])
+    for t in (ti[:rows], ent[:rows]):
+        t[rows - 1] = t[base - 1]
+        t = t.view(rows // base, base, -1)
+        assert (t == t[0]).all()
+    second = (some[:, 1] > some[:, 0]).int()
+    assert (ti[:base, 0] == second).all() and (ti[:base, 1] == 1 - second).all()
+    _close(ent[:base].cpu().numpy(), ref.score(some.double().cpu().numpy(), np.zeros((base, 0), int), 1, "logits")[1], 64 * EPS)

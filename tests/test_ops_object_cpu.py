@@ -23,7 +23,7 @@ def test_the_object_finds_what_it_needs():
     """all symbols bound at once, as the library loads it; the table is complete"""
     capi.load()
     table = C.CDLL(OBJECT, mode=os.RTLD_NOW).lcrc_ops_table
-    table.restype = C.POINTER(C.c_void_p * 6)
+    table.restype = C.POINTER(C.c_void_p * 7)
     assert all(table().contents)
 
 
