@@ -554,10 +554,18 @@ class Lcrc:
         mel = np.ascontiguousarray(mel, dtype=np.float32).reshape(-1, self.nbanks)
         off = np.ascontiguousarray(off, dtype=np.int32)
         rows = mel.shape[0]
+        if off.ndim != 1 or len(off) < 1 or off[-1] != rows:
+            raise LcrcError(LCRC_E_ARG, "posteriors_scored: off must end at the number of frames, %d" % rows)
         m = 0
         if labels is not None:
-            labels = np.ascontiguousarray(labels, dtype=np.int32).reshape(rows, -1)
+            labels = np.asarray(labels)
+            if labels.size % max(rows, 1) or (rows == 0 and labels.size):
+                raise LcrcError(LCRC_E_ARG, "posteriors_scored: %d labels for %d frames" % (labels.size, rows))
+            # (clipped, not wrapped: a label beyond the classes stays beyond them)
+            labels = np.ascontiguousarray(np.clip(labels, -1, 2 ** 31 - 1).astype(np.int32)).reshape(rows, labels.size // max(rows, 1))
             m = labels.shape[1]
+        if not 0 <= k <= 64 or m > 64:
+            raise LcrcError(LCRC_E_ARG, "posteriors_scored: k and the labels of a frame are 0 .. 64")
         out = dict(post=np.zeros((rows, self.n_out), np.float32), entropy=np.zeros(rows, np.float32), logp=np.zeros((rows, m), np.float32),
                    top_index=np.zeros((rows, max(k, 0)), np.int32), top_logp=np.zeros((rows, max(k, 0)), np.float32))
         p = {n: a.ctypes.data for n, a in out.items()}

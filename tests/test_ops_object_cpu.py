@@ -83,3 +83,35 @@ def test_sizes_beyond_a_grid_are_refused():
     assert linear(1 << 30, 128, 128) == over and linear((1 << 30) - 1024, 128, 128) == under
     assert linear(129, 1, 128 * 7400000) == over              # 9 x 7.4 million tiles of 16 x 128, but 3 x 7.4 million of 64 x 128
     assert linear(129, 1, 128 * 5500000) == under
+
+
+def test_posteriors_scored_checks_what_it_hands_over():
+    """offsets that leave the features, labels that do not go by frames or would wrap, lists without an end: nothing reaches the library"""
+    import numpy as np
+    import pytest
+
+    class Library:
+        calls = []
+
+        def lcrc_posteriors_scored(self, h, mel, off, n, post, labels, m, k, *out):
+            self.calls.append(np.ctypeslib.as_array(C.cast(labels, C.POINTER(C.c_int)), (4 * m,)).tolist() if m else [])
+            return 0
+
+    ctx = capi.Lcrc.__new__(capi.Lcrc)
+    ctx.L, ctx.h, ctx.nbanks, ctx.n_out = Library(), None, 15, 39
+    mel = np.zeros((4, 15), np.float32)
+    for bad in (dict(off=[0, 5]), dict(off=[0, 3]), dict(off=[]), dict(off=[[0, 4]]), dict(off=[0, 4], labels=[1, 2, 3])):
+        with pytest.raises(capi.LcrcError) as e:
+            ctx.posteriors_scored(mel, **bad)
+        assert e.value.code == capi.LCRC_E_ARG
+    for bad in (dict(k=65), dict(k=-1), dict(k=1 << 40), dict(labels=np.zeros((4, 65)))):
+        with pytest.raises(capi.LcrcError) as e:
+            ctx.posteriors_scored(mel, [0, 4], **bad)
+        assert e.value.code == capi.LCRC_E_ARG
+    with pytest.raises(capi.LcrcError):
+        ctx.posteriors_scored(mel[:0], [0], labels=[1])
+    assert Library.calls == []
+    ctx.posteriors_scored(mel, [0, 4], labels=np.array([2 ** 32 + 1, -2 ** 40, 7, 2 ** 31 - 1]))
+    ctx.posteriors_scored(mel[:0], [0], labels=np.zeros((0, 3)))
+    assert Library.calls == [[2 ** 31 - 1, -1, 7, 2 ** 31 - 1], []]
+    ctx.h = None
