@@ -248,11 +248,9 @@ __device__ __forceinline__ b8 to_bf16(const i8 &q, int s, float scale)
 // a block's scale from its byte; 255 is no number
 __device__ __forceinline__ float block_scale(int byte) { return byte == 255 ? NAN : __int_as_float(byte << 23); }
 
-// acc += A B over one block of 128 columns; as / bs: the block's scale byte of the lane's row, in the low byte
-template <bool EXACT>
-__device__ __forceinline__ f4 block_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
+// acc += A B over one block of 128 columns with sums in 32 bits; as / bs: the block's scale byte of the lane's row, in the low byte
+__device__ __forceinline__ f4 exact_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
 {
-    if constexpr (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, as, 0, bs);
     const float sa = block_scale(as & 255), sb = block_scale(bs & 255);
 #pragma unroll
     for (int s = 0; s < 4; s++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a, s, sa), to_bf16(b, s, sb), acc, 0, 0, 0);
@@ -367,7 +365,7 @@ __device__ __forceinline__ void copy_to_lds(const unsigned char *base, unsigned 
 template <bool EXACT, int J>
 __device__ __forceinline__ f4 scaled_product(const i8 &a, const i8 &b, f4 acc, int as, int bs)
 {
-    if constexpr (EXACT) return block_product<true>(a, b, acc, as >> (8 * J), bs >> (8 * J));
+    if constexpr (EXACT) return exact_product(a, b, acc, as >> (8 * J), bs >> (8 * J));
     else return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, J, as, J, bs);
 }
 

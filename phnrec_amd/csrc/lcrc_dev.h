@@ -178,7 +178,7 @@ struct SoftmaxRowsParams {
     const float *in;     // [n_rows][n], tight
     float *out;          // row r at out + r * out_ld
     long out_ld;
-    int n_rows, n;       // n <= 1024
+    int n_rows, n;       // n <= 256
     int out_func[2];
     float out_c[2][4];
     float out_l[2][2];

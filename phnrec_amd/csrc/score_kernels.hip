@@ -413,23 +413,22 @@ struct Team {
         return v;
     }
     // The k best of the team's values, best first: out(rank, key), by the thread that finds it.
-    //   first          the bests (value, chunk) of this thread's shares, as keys, 0 where it has none
+    //   first          the best (value, chunk) of this thread's share, as a key, 0 where it has none
     //   scan(bar, f)   f(live, value, chunk, column) for what this thread holds, at least for the values whose keys reach the
     //                  bar; by a whole wave together where the team is one
     //   again(f)       the same for all that it holds, any number of times
-    // The threads' shares are put into 64 G groups.  The k-th best of the groups' bests is reached by at least k values, so
+    // The threads are put into 64 G groups.  The k-th best of the groups' bests is reached by at least k values, so
     // the k best are among the values that reach it, and only threads with such a group look at their values again.  With
     // 256 groups some 74 of random values remain for k = 64, 17 for k = 16 (from 64 groups 300 and 18).  They are ranked by
     // counting.  Rows made so that more remain than fit are done one rank after another.
-    template <int N, typename Scan, typename Again, typename Out>
-    __device__ __forceinline__ void top(int k, const u64 (&first)[N], const Scan &scan, const Again &again, const Out &out)
+    template <typename Scan, typename Again, typename Out>
+    __device__ __forceinline__ void top(int k, u64 first, const Scan &scan, const Again &again, const Out &out)
     {
-        static_assert(N == 1 || T == 64, "a workgroup's threads are groups of one share each");
-        constexpr int G = T > 64 ? 4 : N;
+        constexpr int G = T > 64 ? 4 : 1;
         u64 group[G];
         if (!TOGETHER && t == 0) sh.count = 0;
         if constexpr (T > 64) {
-            sh.best[t] = first[0];
+            sh.best[t] = first;
             sync();
 #pragma unroll
             for (int q = 0; q < G; q++) {
@@ -437,8 +436,7 @@ struct Team {
                 for (int w = q; w < kWaves; w += G) group[q] = max(group[q], sh.best[64 * w + (t & 63)]);
             }
         } else {
-#pragma unroll
-            for (int q = 0; q < G; q++) group[q] = first[q];
+            group[0] = first;
             sync();
         }
         const u64 bar = bar_of(group, k);
@@ -448,10 +446,7 @@ struct Team {
         };
         int n = 0;
         if constexpr (!TOGETHER) {
-            bool look = false;
-#pragma unroll
-            for (int q = 0; q < N; q++) look = look || (first[q] >= bar && first[q] != 0);
-            if (look)
+            if (first >= bar && first != 0)
                 scan(bar, [&](bool live, float v, int chunk, int c) {
                     if (live && reaches(v, chunk)) {
                         const int at = atomicAdd(&sh.count, 1);      // (any order: they are ranked by their keys)
@@ -507,7 +502,7 @@ __device__ __forceinline__ void put_top(const lcrc_score_args &a, size_t r, cons
 }
 
 // ---- a wave to a row, the row in its registers: a chunk of 16 bytes to a lane (rows of up to 64 chunks, k beyond the lists') ----
-// Bound by the fixed part of the search (bar, ballots, ranks): 524288 x 186 f32 with 20 best 330 us.
+// Bound by the fixed part of the search (bar, ballots, ranks): 524288 x 186 f32 with 20 best 297 us.
 template <typename X, bool PROBS>
 __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_args a)
 {
@@ -543,7 +538,7 @@ __global__ __launch_bounds__(kThreads) void score_wave_kernel(const lcrc_score_a
             if (lane < a.k) put_bad(a, r, lane);
             continue;
         }
-        const u64 first[1] = {from < W ? make_key(most, lane) : 0};
+        const u64 first = from < W ? make_key(most, lane) : 0;
         const auto scan = [&](const auto &f) {
 #pragma unroll
             for (int i = 0; i < W; i++) f(i >= from, raw[i], lane, start + i);
@@ -670,7 +665,7 @@ __global__ __launch_bounds__(kThreads) void score_long_kernel(const lcrc_score_a
                     if (c + u * T < to) look_at(raw[u], c + u * T, f);
             }
         };
-        const u64 first[1] = {most_at < 0 ? 0 : make_key(most, most_at)};
+        const u64 first = most_at < 0 ? 0 : make_key(most, most_at);
         team.top(a.k, first, scan, [&](const auto &f) { scan(0, f); }, [&](int rank, u64 key) {
             if (p.parts == 1) put_top<PROBS>(a, r, row, rank, key);
             else list[rank] = key;
@@ -718,8 +713,8 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
                 if (list >= p.parts) list -= p.parts, rank++;
             }
         };
-        u64 first[1] = {};
-        each([&](u64 key) { first[0] = max(first[0], key); });
+        u64 first = 0;
+        each([&](u64 key) { first = max(first, key); });
         const auto scan = [&](u64, const auto &f) {
             each([&](u64 key) { f(key != 0, key_value(key), key_column(key), key_column(key)); });
         };
@@ -730,6 +725,9 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(const lcrc_score_a
 // ---- which kernel, on what grid ----
 int most_blocks = 1 << 22;               // beyond it the workgroups take several rows each (lcrc_debug_score_blocks)
 
+// Lists of 1, 3, 5 and 8 best and seven lengths of rows, since what a row does not need is not free (524288 rows f32, us; in the
+// next longer list or length): 138 columns, 1 best 67 (76), 3 best 81 (97), 5 best 105 (162); lengths of 24 and 48 chunks: 80
+// columns with 5 best 69 (77), 138 columns 105 (126), 300 columns bf16 162 (245).
 template <typename X, bool PROBS, int W, int J>
 void launch_short(const lcrc_score_args &a, int k, hipStream_t stream)
 {

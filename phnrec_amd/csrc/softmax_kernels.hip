@@ -8,8 +8,8 @@
 
 namespace phnrec {
 
-// One wave per row, four rows per workgroup; a row's outputs in registers.
-template <int J>
+// One wave per row, four rows per workgroup; a row's outputs in registers: up to 256 (a merger has at most 208, mlp_supports).
+constexpr int J = 4;
 __global__ __launch_bounds__(256) void softmax_rows_kernel(const SoftmaxRowsParams p)
 {
     const int lane = threadIdx.x & 63;
@@ -42,9 +42,8 @@ __global__ __launch_bounds__(256) void softmax_rows_kernel(const SoftmaxRowsPara
 hipError_t softmax_rows_launch(const SoftmaxRowsParams &p, hipStream_t stream)
 {
     const int blocks = (p.n_rows + 3) / 4;
-    if (p.n <= 256) softmax_rows_kernel<4><<<blocks, 256, 0, stream>>>(p);
-    else if (p.n <= 1024) softmax_rows_kernel<16><<<blocks, 256, 0, stream>>>(p);
-    else return hipErrorInvalidValue;
+    if (p.n > 64 * J) return hipErrorInvalidValue;
+    softmax_rows_kernel<<<blocks, 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
