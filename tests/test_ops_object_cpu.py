@@ -115,3 +115,21 @@ def test_posteriors_scored_checks_what_it_hands_over():
     ctx.posteriors_scored(mel[:0], [0], labels=np.zeros((0, 3)))
     assert Library.calls == [[2 ** 31 - 1, -1, 7, 2 ** 31 - 1], []]
     ctx.h = None
+
+
+def test_no_kernel_has_packed_f32_instructions(tmp_path):
+    """v_pk_add / _mul / _fma_f32, which the compiler makes of ordinary float code where nothing forbids it: some of their forms have
+    given wrong results now and then"""
+    import pytest
+    llvm = "/opt/rocm/llvm/bin/"
+    objects = [os.path.join(ROOT, "phnrec_amd", "lib", "obj", n + ".o")
+               for n in ("lcrc_kernels", "traps_kernels", "phndec_kernels", "frontend_kernels", "score_kernels", "fp8_kernels", "softmax_kernels")]
+    if not all(os.path.exists(p) for p in objects + [llvm + "llvm-objdump", llvm + "clang-offload-bundler"]):
+        pytest.skip("no objects of a build, or no tools to look into them")
+    for p in objects:
+        fat, code = str(tmp_path / "fat"), str(tmp_path / "code")
+        subprocess.run(["objcopy", "-O", "binary", "--only-section=.hip_fatbin", p, fat], check=True)
+        subprocess.run([llvm + "clang-offload-bundler", "--unbundle", "--type=o", "--input=" + fat, "--output=" + code,
+                        "--targets=hipv4-amdgcn-amd-amdhsa--gfx950"], check=True)
+        text = subprocess.check_output([llvm + "llvm-objdump", "-d", code], text=True)
+        assert text.count("\n") > 1000 and not [l for l in text.splitlines() if "v_pk_" in l and "_f32 " in l and "cvt" not in l][:3], p

@@ -12,7 +12,7 @@ if [ "$REF" = "WORKTREE" ]; then
 else
     git -C "$ROOT" archive "$REF" phnrec_amd/csrc include | tar -x -C "$TMP"
 fi
-make -s -C "$TMP/phnrec_amd/csrc" ../lib/libphnrec_lcrc.so HIPFLAGS="-O3 -std=c++17 -fPIC -Wall -Wno-unused-function --offload-arch=gfx950 -ffp-contract=off -mllvm -amdgpu-mfma-vgpr-form $*" 2>&1 | grep -E "error" || true
+make -s -C "$TMP/phnrec_amd/csrc" ../lib/libphnrec_lcrc.so HIPFLAGS="-O3 -std=c++17 -fPIC -Wall -Wno-unused-function --offload-arch=gfx950 -ffp-contract=off -mllvm -amdgpu-mfma-vgpr-form -Xclang -target-feature -Xclang -packed-fp32-ops $*" 2>&1 | grep -E "error" || true
 mkdir -p "$ROOT/phnrec_amd/lib/ab"
 cp "$TMP/phnrec_amd/lib/libphnrec_lcrc.so" "$ROOT/phnrec_amd/lib/ab/lib$NAME.so"
 rm -rf "$TMP"
