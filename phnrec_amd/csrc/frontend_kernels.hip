@@ -38,7 +38,7 @@ __device__ __forceinline__ float alaw_to_linear(unsigned b)
 // logf.  glibc's (2.28 and later; sysdeps/ieee754/flt-32/e_logf.c) is a fixed sequence of IEEE double operations -- a
 // 16-entry table (1/c, ln c), a cubic in double, ONE rounding to float -- and exists in two builds that glibc selects
 // between at load time: with fused multiply-adds and without.  Both sequences are restated here in the device's IEEE
-// double arithmetic (the table and coefficients are glibc's __logf_data, as in host/veclog.cpp); the caller says which
+// double arithmetic (table and coefficients as in host/veclog.cpp); the caller says which
 // one its libm matches (lcrc_frontend_set_ln; the CLI finds out by checking 300 000 values, host/veclog.cpp) and gets that
 // libm's bits.  Form 0 -- log() in double, rounded once -- stays the default of the C entry points: correctly rounded, i.e.
 // glibc's result except where glibc's own 0.818-ulp error shows (about one value in 10^5).

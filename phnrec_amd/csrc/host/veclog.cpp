@@ -21,8 +21,10 @@ namespace phnrec {
 
 namespace {
 
-// glibc's __logf_data (LOGF_TABLE_BITS = 4, LOGF_POLY_ORDER = 4); read out of libm.so.6 of glibc 2.35 and equal to the
-// published table of ARM's optimized-routines, which glibc took it from
+// The table and the polynomial that ARM's optimized-routines publish for logf (math/logf_data.c, 16 intervals, order 4), which
+// glibc's e_logf.c uses too: it has to be the same for the results to be the same bits.  1 / c for a c of every interval -- its
+// middle less 2^-25, or 2^-24 above 1; 1 itself in the interval that holds it, and 1.0534 in the one above, for the accuracy
+// there -- and ln c, each rounded to the nearest double (tests/test_ln_table_cpu.py computes them)
 const double kInvC[16] = {0x1.661ec79f8f3bep+0, 0x1.571ed4aaf883dp+0, 0x1.49539f0f010bp+0,  0x1.3c995b0b80385p+0,
                           0x1.30d190c8864a5p+0, 0x1.25e227b0b8eap+0,  0x1.1bb4a4a1a343fp+0, 0x1.12358f08ae5bap+0,
                           0x1.0953f419900a7p+0, 0x1p+0,               0x1.e608cfd9a47acp-1, 0x1.ca4b31f026aap-1,
