@@ -196,6 +196,8 @@ int lcrc_set_kernel_done_callback(lcrc_ctx *ctx, lcrc_kernel_done_fn fn, void *a
  * library keeps nothing between calls and allocates nothing inside them: scratch memory is the caller's (`workspace`, its
  * size from the function named beside it, aligned to 16 bytes), used from the call's start to the end of its work on the
  * stream -- calls that may overlap on the device, captured graphs among them, need one each.  All calls may be captured.
+ * Their kernels are an object of their own, libphnrec_lcrc_ops.so, which the first call that launches one loads from this
+ * library's folder (LCRC_E_DEVICE where it is not there).
  * Errors: a negative code, text in lcrc_last_error(NULL).  Sizes of 0 rows are no-ops.  An argument structure is read
  * during the call only.  Results do not depend on what else runs, and are the same in every run. */
 enum { LCRC_T_F32 = 0, LCRC_T_F16 = 1, LCRC_T_BF16 = 2, LCRC_T_E4M3 = 3 };

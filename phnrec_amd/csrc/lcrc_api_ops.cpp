@@ -30,8 +30,8 @@ struct DeviceScope {
     }
 };
 
-// The kernels' object (ops_dev.h), which lies beside this library; NULL and a text where it cannot be had.  Loaded once, by the
-// first call that launches something, and never unloaded.
+// The kernels' object (ops_dev.h); NULL and a text where it cannot be had.  Loaded once, by the first call that launches something,
+// and never unloaded.  It lies beside this library: the library's own search path is its folder, as it was when it was loaded.
 const OpsTable *ops(std::string *why)
 {
     struct Loaded {
@@ -39,15 +39,11 @@ const OpsTable *ops(std::string *why)
         std::string error;
         Loaded()
         {
-            Dl_info here;
-            if (!dladdr(reinterpret_cast<const void *>(&lcrc_score), &here) || !here.dli_fname) { error = "cannot find this library's folder"; return; }
-            std::string path = here.dli_fname;
-            const size_t slash = path.rfind('/');
-            path = (slash == std::string::npos ? std::string() : path.substr(0, slash + 1)) + "libphnrec_lcrc_ops.so";
-            void *const object = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+            void *const object = dlopen("libphnrec_lcrc_ops.so", RTLD_NOW | RTLD_LOCAL);
             const auto table_of = object ? reinterpret_cast<const OpsTable *(*)()>(dlsym(object, "lcrc_ops_table")) : nullptr;
-            if (table_of) table = table_of();
-            else { const char *e = dlerror(); error = e ? e : path; }
+            if (!table_of) { const char *e = dlerror(); error = e ? e : "libphnrec_lcrc_ops.so"; return; }
+            if (table_of()->version == kOpsVersion) table = table_of();
+            else error = "libphnrec_lcrc_ops.so is of another build";
         }
     };
     static const Loaded loaded;

@@ -120,8 +120,11 @@ constexpr long long kQMaxTiles = 1ll << 26;      // a matrix in the 8-bit form, 
 constexpr int kQMaxIn = 1 << 23;      // columns of the operands of a product: their tiles' offsets stay within 32 bits
 
 // ---- the kernels' object ----------------------------------------------------------------------------------------------
-// Its one exported symbol, lcrc_ops_table, gives the launches.
+// Its one exported symbol, lcrc_ops_table, gives the launches.  The version goes up with every change of the table or of the
+// structures it hands over.
+constexpr int kOpsVersion = 2;
 struct OpsTable {
+    int version;
     hipError_t (*score)(const lcrc_score_args &a, hipStream_t stream);
     hipError_t (*fp8_pack)(const Fp8PackParams &p, hipStream_t stream);
     hipError_t (*fp8_unpack)(const Fp8UnpackParams &p, hipStream_t stream);

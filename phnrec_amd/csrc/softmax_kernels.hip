@@ -52,7 +52,7 @@ hipError_t softmax_rows_launch(const SoftmaxRowsParams &p, hipStream_t stream)
 // the launches of this object (ops_dev.h)
 extern "C" __attribute__((visibility("default"))) const phnrec::OpsTable *lcrc_ops_table()
 {
-    static const phnrec::OpsTable table = {phnrec::score_launch, phnrec::fp8_pack_launch, phnrec::fp8_unpack_launch, phnrec::fp8_product_launch,
+    static const phnrec::OpsTable table = {phnrec::kOpsVersion, phnrec::score_launch, phnrec::fp8_pack_launch, phnrec::fp8_unpack_launch, phnrec::fp8_product_launch,
                                            phnrec::fp8_few_rows_launch, phnrec::softmax_rows_launch, phnrec::score_most_blocks};
     return &table;
 }

@@ -23,8 +23,39 @@ def test_the_object_finds_what_it_needs():
     """all symbols bound at once, as the library loads it; the table is complete"""
     capi.load()
     table = C.CDLL(OBJECT, mode=os.RTLD_NOW).lcrc_ops_table
-    table.restype = C.POINTER(C.c_void_p * 7)
+    table.restype = C.POINTER(C.c_void_p * 8)                # (version, seven launches)
     assert all(table().contents)
+
+
+MOVED = """
+import ctypes as C, os, sys
+C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+os.chdir(sys.argv[2])
+L = C.CDLL("./libphnrec_lcrc.so")
+os.chdir("/")
+L.lcrc_last_error.restype = C.c_char_p
+print(L.lcrc_debug_score_blocks(1 << 22), L.lcrc_last_error(None).decode())
+"""
+
+
+def test_the_object_is_found_beside_the_library(tmp_path):
+    """loaded by a relative path, from another folder afterwards; missing; of another build"""
+    import shutil
+    stub = str(tmp_path / "stub.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-w", "-o", stub, os.path.join(ROOT, "tests", "hip_stub.c"), "-lpthread"], check=True)
+
+    def said(folder):
+        return subprocess.check_output([sys.executable, "-c", MOVED, stub, folder], text=True)
+
+    here = tmp_path / "lib"
+    here.mkdir()
+    shutil.copy(capi.LIB_PATH, str(here))
+    assert said(str(here)).startswith("-4 cannot load the operators' kernels") and "libphnrec_lcrc_ops.so" in said(str(here))
+    shutil.copy(OBJECT, str(here))
+    assert said(str(here)).startswith("%d " % (1 << 22))
+    (tmp_path / "o.c").write_text("static const long table[8] = {1}; const void *lcrc_ops_table(void) { return table; }")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(here / "libphnrec_lcrc_ops.so"), str(tmp_path / "o.c")], check=True)
+    assert "another build" in said(str(here))
 
 
 def test_refusals_and_sizes_do_not_load_it():
