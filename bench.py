@@ -432,6 +432,12 @@ def synthetic_list(td, n_files, seed=1236, rate=8000):
 SETTLE_S = 0.3
 
 
+def list_loop_seconds(kv):
+    """the list loop while contexts work on it, from a PHNREC_STATS line's figures (milliseconds: a short list can be done within
+    the one in which its first context came up)"""
+    return max(1e-3, float(kv["wall_s"]) - float(kv.get("first_ctx_s", 0)))
+
+
 def run_cli(exe, args, env, timeout=600):
     """one CLI run: wall clock of the process and the figures of its PHNREC_STATS line"""
     import subprocess
@@ -449,7 +455,7 @@ def run_cli(exe, args, env, timeout=600):
     # contexts work on it: frames / (wall_s - first_ctx_s) --, `setup_s` what lies in front of the first launch, and
     # `process_frames_per_s` (exec to exit) is the figure a caller of the CLI sees.
     first_ctx = float(kv.get("first_ctx_s", 0))
-    loop_s = max(1e-6, float(kv["wall_s"]) - first_ctx)
+    loop_s = list_loop_seconds(kv)
     return {"value": round(float(kv["frames"]) / loop_s, 1), "unit": "frames/s", "list_wall_s": round(loop_s, 3),
             "list_from_first_line_s": float(kv["wall_s"]), "first_ctx_s": first_ctx, "contexts": int(kv.get("contexts", 0)),
             "process_wall_s": round(wall, 3), "xrt": float(kv["xRT"]), "gpu_kernel_ms": float(kv["gpu_kernel_ms"]),
@@ -804,7 +810,7 @@ def four_systems_leg(n_gpus, dmap, n_files=2500, variants=None):
                     nf = int(kv["files"])
                     name = systems[3] if nf == n_files else systems[n_files - 1 - nf]
                     # (the list loop while contexts work on it, as in run_cli: wall_s minus the time until the first context was up)
-                    loop_s = max(1e-6, float(kv["wall_s"]) - float(kv.get("first_ctx_s", 0)))
+                    loop_s = list_loop_seconds(kv)
                     per[name] = {"files": nf, "frames": int(kv["frames"]), "frames_per_s": round(int(kv["frames"]) / loop_s, 1),
                                  "list_wall_s": round(loop_s, 3), "first_ctx_s": float(kv.get("first_ctx_s", 0)),
                                  "main_s": float(kv["main_s"]), "xrt": float(kv["xRT"]), "contexts": int(kv.get("contexts", 0)),
