@@ -77,7 +77,6 @@ static int NextOpt(int argc, char **argv, const char *options, int &ind, const c
     return 1;
 }
 
-static SpeechRec *g_sr = nullptr;
 
 // peak resident set of this process so far (PHNREC_STATS prints it: pinned buffers count)
 // (pinned buffers included, also where the resident set does not count them; they are as large as they ever were, since the
@@ -109,29 +108,10 @@ static std::string RssKinds()
     return out;
 }
 
-// The process ends without tearing the HIP runtime down piece by piece (contexts, streams, pinned buffers, code objects: tens of
-// milliseconds that a one-file run would notice, with the runtime's own threads beside it); the driver reclaims it all.
-// Profilers, which live on exit handlers, get the ordinary exit.  Any other preloaded library does not: a run that has one
-// would otherwise go through a tear-down that no other run goes through.
-static void LeaveAtOnce(int code)
-{
-    fflush(NULL);                            // every open output stream, not only stdout / stderr
-#if !defined(__SANITIZE_ADDRESS__) && !defined(__SANITIZE_THREAD__) && !defined(PHNREC_COVERAGE)
-    const auto named = [](const char *e) { return e && *e; };
-    const char *preload = getenv("LD_PRELOAD");
-    if (!named(getenv("ROCP_TOOL_LIBRARIES")) && !named(getenv("HSA_TOOLS_LIB")) && !named(getenv("PHNREC_CLEAN_EXIT")) &&
-        !(preload && strstr(preload, "rocprof")))
-        _Exit(code);
-#else
-    (void)code;                              // (sanitizer and coverage builds report from exit handlers)
-#endif
-}
-
 static void Die(const std::string &msg)
 {
     fprintf(stderr, "ERROR: %s", msg.c_str());
     if (msg.empty() || msg.back() != '\n') fputc('\n', stderr);
-    LeaveAtOnce(1);
     exit(1);
 }
 
@@ -256,7 +236,6 @@ int main(int argc, char **argv)
         if (lcrc_debug_fail_launch(atoi(e)) != LCRC_OK) Die(std::string(lcrc_last_error(nullptr)) + "\n");
 
     SpeechRec SR;
-    g_sr = &SR;
     SR.SetVerbose(verbose);
     if (!config_dir) Die("Configuration directory is not set (-c)\n");
     SR.SetGpus(gpus);
@@ -312,7 +291,15 @@ int main(int argc, char **argv)
                 s.cpu_stage1 + s.cpu_read + s.cpu_gather + s.cpu_stage3, s.cpu_stage1, s.cpu_read, s.cpu_gather, s.cpu_stage3, s.cpu_viterbi,
                 s.host_threads, s.contexts, SR.ModeString().c_str(), MaxRssMb(), RssKinds().c_str());
     }
-    // every output file is closed by now
-    LeaveAtOnce(0);
-    return 0;
+    // Every output file is closed by now.  Leave without tearing the HIP runtime down piece by piece (contexts, streams,
+    // pinned buffers, code objects: tens of milliseconds that a one-file run would notice); the driver reclaims it all.
+    // (tools that live on exit handlers -- rocprofv3 and other preloaded profilers -- get the ordinary exit)
+    fflush(NULL);                            // every open output stream, not only stdout / stderr
+#if defined(__SANITIZE_ADDRESS__) || defined(__SANITIZE_THREAD__) || defined(PHNREC_COVERAGE)
+    return 0;                                // sanitizer / coverage builds report from exit handlers
+#else
+    const auto named = [](const char *e) { return e && *e; };
+    if (named(getenv("LD_PRELOAD")) || named(getenv("ROCP_TOOL_LIBRARIES")) || named(getenv("HSA_TOOLS_LIB")) || named(getenv("PHNREC_CLEAN_EXIT"))) return 0;
+    _Exit(0);
+#endif
 }

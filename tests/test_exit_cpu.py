@@ -1,5 +1,5 @@
-"""How the command line leaves: at once after its outputs are closed, or by the ordinary return where a profiler lives on exit
-handlers.  A variable that is set but empty, and any other preloaded library, change nothing."""
+"""How the command line leaves: at once after its outputs are closed, or by the ordinary return where a preloaded tool may live
+on exit handlers.  A tool that is not there -- a variable that is set but empty -- does not count."""
 import os
 import subprocess
 
@@ -12,33 +12,17 @@ BIN = os.path.join(ROOT, "phnrec_amd", "bin", "phnrec")
 
 @pytest.mark.parametrize("name,value,ordinary", [(None, None, False), ("LD_PRELOAD", "", False), ("ROCP_TOOL_LIBRARIES", "", False),
                                                  ("HSA_TOOLS_LIB", "", False), ("PHNREC_CLEAN_EXIT", "", False),
-                                                 ("LD_PRELOAD", "libm.so.6", False), ("PHNREC_CLEAN_EXIT", "1", True)])
+                                                 ("LD_PRELOAD", "libm.so.6", True), ("PHNREC_CLEAN_EXIT", "1", True)])
 def test_ordinary_exit_only_for_a_tool_that_is_named(tmp_path, name, value, ordinary):
     if os.environ.get("LD_PRELOAD"):
         pytest.skip("something is preloaded here")
     env = {k: v for k, v in os.environ.items() if k not in ("LD_PRELOAD", "ROCP_TOOL_LIBRARIES", "HSA_TOOLS_LIB", "PHNREC_CLEAN_EXIT")}
     if name:
         env[name] = value
-    # (the loader reports the end of every object, unless the process leaves without exit handlers)
+    # the loader reports the end of every object, unless the process leaves without exit handlers
     p = subprocess.run([BIN, "-c", model_dir("PHN_HU_SPDAT_LCRC_N1500"), "-i", os.path.join(GOLD, "test.raw"), "-t", "par", "-o",
                         str(tmp_path / "o")], env=dict(env, LD_DEBUG="files"), capture_output=True, text=True)
     assert p.returncode == 0 and ("calling fini" in p.stderr) == ordinary
-
-
-def test_a_profiler_gets_the_ordinary_exit(tmp_path):
-    tool = str(tmp_path / "librocprof_stand_in.so")
-    subprocess.run(["gcc", "-shared", "-fPIC", "-x", "c", "/dev/null", "-o", tool], check=True)
-    if os.environ.get("LD_PRELOAD"):
-        pytest.skip("something is preloaded here")
-    for args, code in ((["-t", "par"], 0), (["-t", "nonsense"], 1)):
-        p = subprocess.run([BIN, "-c", model_dir("PHN_HU_SPDAT_LCRC_N1500"), "-i", os.path.join(GOLD, "test.raw"), "-o", str(tmp_path / "o")] + args,
-                           env=dict(os.environ, LD_DEBUG="files", LD_PRELOAD=tool), capture_output=True, text=True)
-        assert p.returncode == code and "calling fini" in p.stderr
-
-
-def test_an_error_leaves_at_once_too(tmp_path):
-    p = subprocess.run([BIN, "-t", "nonsense"], env=dict(os.environ, LD_DEBUG="files"), capture_output=True, text=True)
-    assert p.returncode == 1 and "Invalid data format" in p.stderr and "calling fini" not in p.stderr
 
 
 def test_a_crash_names_its_place(tmp_path):
