@@ -248,7 +248,8 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
 /* y = act(x W^T + bias), x[rows][n_in] and W[n_out][n_in] (NeuralNet's layout, nn.cpp:702-740) in the 8-bit form: exact
  * products of the held values, added up in 32 bits.  (Held values below 2^-126 may count as zeros, of 2^128 and above as
  * infinite.  Where y is bf16 the 8-bit matrix instructions cut off, inside each group of eight products, what lies 13 bits below
- * the largest of them: at most 7 * 2^-13 of sum |x w|, a fifth of a rounding to bf16.)  x is a matrix in that form (LCRC_T_E4M3,
+ * the largest of them: at most 7 * 2^-13 of sum |x w|, a fifth of a rounding of that sum to bf16; for terms that nearly cancel
+ * one another take f16 or f32.)  x is a matrix in that form (LCRC_T_E4M3,
  * ldx ignored) or is put into it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32,
  * f16 or bf16 rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
  * n_in <= 2^23; W, x and y hold fewer than 2^26 tiles of 16 rows x 128 columns (so does a matrix that is packed or unpacked),

@@ -120,7 +120,7 @@ struct RawBlock {
     }
 };
 
-// One wave per tile of 16 rows x 128 columns: 8192 x 8192 bf16 in 46 us, 4.4 TB/s.  NORM: the values are normalised first, (v - mean[column]) * dev[column]
+// One wave per tile of 16 rows x 128 columns: 8192 x 8192 bf16 in 41 us, 4.9 TB/s.  NORM: the values are normalised first, (v - mean[column]) * dev[column]
 // (Normalize, nn.cpp:702-716).
 template <typename X, bool NORM = false>
 __global__ __launch_bounds__(256) void fp8_pack_kernel(const Fp8PackParams p)
@@ -223,11 +223,12 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
 // The 8-bit matrix instructions multiply exactly, but inside a group of eight products (eight bytes of a lane that follow one
 // another) they cut every product off 13 bits below the group's largest one before they add (measured, for the scaled and the
 // plain form alike: 2^16 + 3 * 2^3 comes out whole, of 2^16 + 3 * 7 the sevens are gone); the groups' sums are added in 32
-// bits.  That is up to 7 * 2^-13 = 0.22 * 2^-8 of the products' absolute sum, 1.4e-5 relative on normal values: beside the
-// rounding of a result to bf16, 2^-8, a fifth at the very most, in 3 of 1000 results the other neighbour.  It is more than f16's
-// rounding, 2^-11; too much for a result in 32 bits; and for one in 8, whose rounding turns 1.4e-5 into a whole step, 2^-3,
-// wherever it lies that near to a border: a net with hidden values in 8 bits was off by 5.5e-4 of its results where sums in 32
-// bits leave 2.1e-4.  So products with results in anything but bf16 turn their operands into bf16 --
+// bits.  That is up to 7 * 2^-13 = 0.22 * 2^-8 of the products' absolute sum, 1.4e-5 of it on normal values: beside the rounding
+// of a result to bf16, 2^-8, it changes the neighbour that 4 (276 inputs) to 16 (8192) of 1000 results are rounded to and not
+// their distance from the definition (rms 1.6597e-3 of them, with sums in 32 bits 1.6595e-3).  It is more than f16's rounding,
+// 2^-11; too much for a result in 32 bits; and for one in 8, whose rounding turns 1.4e-5 into a whole step, 2^-3, wherever it
+// lies that near to a border: a net with hidden values in 8 bits was off by 5.5e-4 of its results where sums in 32 bits leave
+// 2.1e-4.  So products with results in anything but bf16 turn their operands into bf16 --
 // exact: 4 significant bits, the block's scale goes into bf16's exponent (v_cvt_scalef32_pk_bf16_fp8; below 2^-126 it loses
 // bits) -- and use the bf16 instruction, whose sums are f32 throughout: half the rate.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -376,11 +377,10 @@ __device__ __forceinline__ void for_each(const F &f, std::integer_sequence<int, 
 }
 
 // A workgroup of WW x WX waves makes 16 FW WW outputs of 16 FX WX rows, each wave FW x FX tiles in its registers.
-// 256 x 128, two workgroups to a CU so that one copies and reads while the other multiplies: 8192^3 to bf16 in 460 - 475 us,
-// 2.3 PFLOP/s (first version, operands straight from memory, 1630).  Without its copies it takes 375 - 407 us, without copies
-// and reads of LDS 330: the copies are what is left.  256 x 256 with a wave to a SIMD: 535 - 570, nothing runs beside its
-// epilogue.  4096 x 2048 x 8192 with bf16 operands (EXACT, 128 x 128): 150 - 160 us.  Small tiles are chains: 777 x 1999 x 2309
-// in 12.6 us is 4 us and sixteen blocks of 0.5; a third stage of LDS changes nothing there.
+// 256 x 128, two workgroups to a CU so that one copies and reads while the other multiplies: 8192^3 to bf16 in 431 - 475 us,
+// 2.3 - 2.55 PFLOP/s (first version, operands straight from memory, 1630; 256 x 256 with a wave to a SIMD 535 - 570, nothing
+// runs beside its epilogue).  With bf16 operands (EXACT, 128 x 128): 8192^3 to f16 901 us, 4096 x 2048 x 8192 140 - 150.  Small
+// tiles are chains of sixteen blocks: 777 x 1999 x 2309 to bf16 14.6 us, to f16 19.5; a third stage of LDS changes nothing there.
 template <bool EXACT, int FW, int FX, int WW, int WX, int STAGES = 1>
 __global__ __launch_bounds__(64 * WW * WX, 2) void fp8_tile_kernel(const Fp8ProductParams p, int across, int down)
 {

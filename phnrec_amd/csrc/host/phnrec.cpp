@@ -78,9 +78,8 @@ static int NextOpt(int argc, char **argv, const char *options, int &ind, const c
 }
 
 
-// peak resident set of this process so far (PHNREC_STATS prints it: pinned buffers count)
-// (pinned buffers included, also where the resident set does not count them; they are as large as they ever were, since the
-// contexts are still there)
+// peak resident set of this process so far (PHNREC_STATS prints it), pinned buffers included, also where the resident set does
+// not count them: they are as large as they ever were, since the contexts are still there
 static double MaxRssMb()
 {
     struct rusage ru;

@@ -21,9 +21,9 @@ constexpr int kScoreMaxTop = 64, kScoreMaxLabels = 64;
 constexpr int kScoreMaxCols = 1 << 30;
 
 // Rows of up to this many chunks of 16 bytes lie in a wave's registers, a chunk to a lane; up to so many a wave streams its
-// row, beyond it a workgroup.  (30000 x 3000 f16, k = 16: streamed by a wave 80 us, 8 chunks to a lane in registers 578, the
-// register file full of keys; 60000 x 1000 f32, k = 5: 74 and 101.  20000 x 4096 f32, k = 8: by a wave 68 us, by a workgroup 109;
-// 12000 x 8192: 80 and 88.)
+// row, beyond it a workgroup.  (30000 x 3000 f16, k = 16: streamed by a wave 77 us, 8 chunks to a lane in registers 578, the
+// register file full of keys; 60000 x 1000 f32, k = 5: 68 and 101.  20000 x 4096 f32, k = 8: by a wave 65 us, by a workgroup 109;
+// 12000 x 8192: 79 and 88.)
 constexpr int kScoreThreads = 256, kScoreHeldChunks = 64, kScoreWaveChunks = 32 * 64;
 
 // a row's cut into parts of so many chunks of 16 bytes, a workgroup to each
@@ -76,7 +76,7 @@ struct Q8Shape {
 // Which kernel makes a product (measured, us): large tiles of outputs x rows read least per product, but need two workgroups for
 // every CU:
 //   4096 x 8192 x 2048 bf16   256 x 128 (256 tiles) 86, 128 x 128 (512) 73, 128 x 64 100
-//   777 x 1999 x 2309 f16     128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
+//   777 x 1999 x 2309 bf16    128 x 128 16.4, 128 x 64 (247) 12.6, shared-out sums 27;  300 x 4000 x 1000 (40): 18, sums 11
 // In short sums nothing is read often enough to count, and small tiles fill the card better:
 //   8192 x 372 x 1500 in 8 bits  128 x 128 26.5, 128 x 64 25.3
 enum Fp8Route { kFp8SharedSums = 0, kFp8Tiles128x64 = 1, kFp8Tiles128x128 = 2, kFp8Tiles256x128 = 3 };
@@ -84,7 +84,7 @@ inline long long fp8_tiles(int rows, int n_out, int tile_outputs, int tile_rows)
 {
     return (((long long)n_out + tile_outputs - 1) / tile_outputs) * (((long long)rows + tile_rows - 1) / tile_rows);
 }
-// (fp8_kernels.hip: what the 8-bit matrix instructions cut off lies below the rounding of a result in bf16, and of no other)
+// (fp8_kernels.hip: what the 8-bit matrix instructions cut off is little beside the rounding of a result in bf16, and of no other)
 inline bool fp8_sums_in_32_bits(int y_type) { return y_type != LCRC_T_BF16; }
 inline Fp8Route fp8_route(int rows, int n_in, int n_out, int y_type)
 {
