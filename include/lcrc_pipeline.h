@@ -91,7 +91,8 @@ int lcrc_wave_to_posteriors(lcrc_ctx *ctx, const unsigned char *bytes, const lon
  * demand inside its first call (device staging, pinned features / posteriors / offsets; with max_wave_bytes > 0 -- after
  * lcrc_frontend_configure -- the byte buffers of the waveform entries too).  Optional: the entry points grow their buffers
  * themselves; page pinning is what that costs (~8 ms per 32 768 HU frames), and a caller with a set-up phase calls this
- * there.  With it launches of that size can be captured into a graph (lcrc_posteriors_device).  Call it after
+ * there.  With it launches of that size can be captured into a graph (lcrc_posteriors_device, without lcrc_set_timing's events
+ * and lcrc_set_launch_order).  Call it after
  * lcrc_set_merger_fp8 and lcrc_decoder_configure / lcrc_set_posterior_readback (they decide whether a pinned posterior
  * buffer is needed at all).  Has no reference counterpart (the reference allocates per bunch, traps.cpp:63-101). */
 int lcrc_reserve(lcrc_ctx *ctx, int max_rows, int max_utts, long long max_wave_bytes);

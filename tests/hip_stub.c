@@ -1,6 +1,6 @@
-/* A stand-in for the HIP runtime, for tests of what the library does around its GPU calls (tests/test_start_up_cpu.py and others):
- * device memory is host memory, copies are done at once, kernels do nothing.  Every call sleeps as long as stub_sleep_us says
- * for its kind and notes which other calls were inside the runtime meanwhile. */
+/* A stand-in for the HIP runtime, for tests of what the library does around its GPU calls (test_start_up_cpu.py and others):
+ * device memory is host memory, copies are done at once, kernels do nothing; it counts launches, allocations and frees, and
+ * says that every stream is captured while stub_capturing is set. */
 #define _GNU_SOURCE
 #include <dirent.h>
 #include <pthread.h>
@@ -14,8 +14,7 @@
 typedef struct { unsigned x, y, z; } dim3;
 typedef int hipError_t;
 
-atomic_int stub_inside, stub_loading, stub_beside_a_load, stub_calls, stub_launches, stub_mallocs, stub_frees, stub_capturing, stub_last_error;
-int stub_load_us = 0;
+atomic_int stub_launches, stub_mallocs, stub_frees, stub_capturing;
 
 static int threads_of_this_process(void)
 {
@@ -43,25 +42,14 @@ static void start_up(void)
     up = 1;
     pthread_mutex_unlock(&mu);
 }
-static void enter(void)
-{
-    start_up();
-    atomic_fetch_add(&stub_calls, 1);
-    atomic_fetch_add(&stub_inside, 1);
-    if (atomic_load(&stub_loading)) atomic_fetch_add(&stub_beside_a_load, 1);
-}
-static hipError_t leave(void)
-{
-    if (atomic_load(&stub_loading)) atomic_fetch_add(&stub_beside_a_load, 1);
-    atomic_fetch_sub(&stub_inside, 1);
-    return 0;
-}
+static void enter(void) { start_up(); }
+static hipError_t leave(void) { return 0; }
 #define PLAIN { enter(); return leave(); }
 
 hipError_t hipGetDeviceCount(int *n) { enter(); *n = 1; return leave(); }
 hipError_t hipSetDevice(int d) { (void)d; PLAIN }
 hipError_t hipGetDevice(int *d) { enter(); *d = 0; return leave(); }
-hipError_t hipGetLastError(void) { return atomic_exchange(&stub_last_error, 0); }
+hipError_t hipGetLastError(void) { return 0; }
 const char *hipGetErrorString(hipError_t e) { (void)e; return "stub error"; }
 static hipError_t get(void **p, size_t n)
 {
@@ -117,17 +105,7 @@ hipError_t hipEventSynchronize(void *e) { (void)e; PLAIN }
 hipError_t hipEventQuery(void *e) { (void)e; PLAIN }
 hipError_t hipEventElapsedTime(float *ms, void *a, void *b) { (void)a; (void)b; enter(); *ms = 1.0f; return leave(); }
 hipError_t hipFuncSetAttribute(const void *f, int a, int v) { (void)f; (void)a; (void)v; PLAIN }
-/* what brings a code object onto the device */
-hipError_t hipFuncGetAttributes(void *a, const void *f)
-{
-    (void)a; (void)f;
-    enter();
-    if (atomic_load(&stub_inside) > 1) atomic_fetch_add(&stub_beside_a_load, 1);
-    atomic_fetch_add(&stub_loading, 1);
-    usleep((unsigned)stub_load_us);
-    atomic_fetch_sub(&stub_loading, 1);
-    return leave();
-}
+hipError_t hipFuncGetAttributes(void *a, const void *f) { (void)a; (void)f; PLAIN }
 hipError_t hipDeviceGetAttribute(int *v, int a, int d) { (void)a; (void)d; enter(); *v = 256; return leave(); }
 hipError_t hipDeviceGetPCIBusId(char *b, int n, int d) { (void)d; enter(); snprintf(b, (size_t)n, "0000:00:00.0"); return leave(); }
 hipError_t hipLaunchKernel(const void *f, dim3 g, dim3 b, void **a, size_t l, void *s)
