@@ -272,3 +272,53 @@ def test_more_short_rows_than_a_grid_has_lanes_for(capi):
     second = (some[:, 1] > some[:, 0]).int()
     assert (ti[:base, 0] == second).all() and (ti[:base, 1] == 1 - second).all()
     _close(ent[:base].cpu().numpy(), ref.score(some.double().cpu().numpy(), np.zeros((base, 0), int), 1, "logits")[1], 64 * EPS)
+
+
+FIRST = """
+import sys
+import numpy as np, torch
+from phnrec_amd import capi
+capi.load()
+rng = np.random.default_rng(1)
+rows, n_in, n_out, k = 40, 300, 500, 5
+f = dict(device="cuda")
+x = torch.from_numpy(rng.standard_normal((rows, n_in)).astype(np.float32)).cuda()
+w = torch.from_numpy(rng.standard_normal((n_out, n_in)).astype(np.float32)).cuda()
+q = torch.zeros(capi.fp8_bytes(n_out, n_in), dtype=torch.uint8, **f)
+y = torch.zeros(rows, n_out, **f)
+ws = torch.zeros(max(capi.fp8_linear_workspace(rows, n_in, 0), 16), dtype=torch.uint8, **f)
+ti, ent = torch.zeros(rows, k, dtype=torch.int32, **f), torch.zeros(rows, **f)
+lin = capi.Fp8LinearArgs(x=x.data_ptr(), x_type=0, rows=rows, n_in=n_in, n_out=n_out, ldx=n_in, w=q.data_ptr(), act=0, y=y.data_ptr(), y_type=0,
+                         ldy=n_out, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+sc = capi.ScoreArgs(x=y.data_ptr(), type=0, form=0, rows=rows, cols=n_out, ld=n_out, k=k, entropy=ent.data_ptr(), top_index=ti.data_ptr())
+def calls():
+    s = torch.cuda.current_stream().cuda_stream
+    capi.fp8_pack(w.data_ptr(), 0, n_out, n_in, n_in, q.data_ptr(), stream=s)
+    capi.fp8_linear(lin, stream=s)
+    capi.score(sc, stream=s)
+assert "lcrc_ops" not in open("/proc/self/maps").read()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+assert "libphnrec_lcrc_ops.so" in open("/proc/self/maps").read()
+for i in range(3):
+    x.normal_(); w.normal_()
+    for t in (q, y, ti, ent): t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in (q, y, ti, ent)]
+    for t in (q, y, ti, ent): t.zero_()
+    calls()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, (q, y, ti, ent))) and float(y.abs().sum()) > 0
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(capi):
+    """the kernels' object and their code are loaded inside the capture"""
+    import subprocess
+    import sys
+    from tests.util import ROOT
+    p = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and p.stdout.split()[-1] == "same", p.stderr[-2000:]
