@@ -92,9 +92,8 @@ int lcrc_wave_to_posteriors(lcrc_ctx *ctx, const unsigned char *bytes, const lon
  * lcrc_frontend_configure -- the byte buffers of the waveform entries too).  Optional: the entry points grow their buffers
  * themselves; page pinning is what that costs (~8 ms per 32 768 HU frames), and a caller with a set-up phase calls this
  * there.  With it launches of that size can be captured into a graph (lcrc_posteriors_device, without lcrc_set_timing's events
- * and lcrc_set_launch_order).  Call it after
- * lcrc_set_merger_fp8 and lcrc_decoder_configure / lcrc_set_posterior_readback (they decide whether a pinned posterior
- * buffer is needed at all).  Has no reference counterpart (the reference allocates per bunch, traps.cpp:63-101). */
+ * and lcrc_set_launch_order).  Call it after lcrc_set_merger_fp8 and lcrc_decoder_configure / lcrc_set_posterior_readback (they
+ * decide whether a pinned posterior buffer is needed at all).  Has no reference counterpart (the reference allocates per bunch, traps.cpp:63-101). */
 int lcrc_reserve(lcrc_ctx *ctx, int max_rows, int max_utts, long long max_wave_bytes);
 /* Zero-copy variant: lcrc_wave_stage_buffer returns the context's pinned byte buffer (valid until a later
  * call asks for more capacity); the caller reads its files straight into it -- utterance u at start[u]
@@ -250,9 +249,9 @@ int lcrc_fp8_unpack(int device_id, const void *src, int rows, int cols, void *ds
  * products of the held values, added up in 32 bits.  (Held values below 2^-126 may count as zeros, of 2^128 and above as
  * infinite.  Where y is bf16 the 8-bit matrix instructions cut off, inside each group of eight products, what lies 13 bits below
  * the largest of them: at most 7 * 2^-13 of sum |x w|, a fifth of a rounding of that sum to bf16; for terms that nearly cancel
- * one another take f16 or f32.)  x is a matrix in that form (LCRC_T_E4M3,
- * ldx ignored) or is put into it by the call (f32, f16, bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32,
- * f16 or bf16 rows, or as a matrix in the 8-bit form (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
+ * one another take f16 or f32.)  x is a matrix in that form (LCRC_T_E4M3, ldx ignored) or is put into it by the call (f32, f16,
+ * bf16 rows; workspace: lcrc_fp8_linear_workspace).  y is written as f32, f16 or bf16 rows, or as a matrix in the 8-bit form
+ * (LCRC_T_E4M3: lcrc_fp8_bytes(rows, n_out) bytes, ldy ignored): the next product's x.
  * n_in <= 2^23; W, x and y hold fewer than 2^26 tiles of 16 rows x 128 columns (so does a matrix that is packed or unpacked),
  * y fewer than 2^24 - 7 of 64 rows x 128 columns, what is begun counting as a whole one.
  * LCRC_ACT_SIGMOID: 1 / (1 + exp(-v)); LCRC_ACT_FSIGMOID: the same with the reference's fast exponential (fexp.h:14-21),

@@ -510,7 +510,8 @@ int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s)
     const size_t fp8 = c->fp8_merger ? merger_fp8_bytes(c, n_rows) : 0;
     const bool more_rows = n_rows > c->cap_feat_rows, more_fp8 = fp8 > c->cap_fp8;
     if (captured && (more_rows || more_fp8))
-        return fail(c, LCRC_E_UNSUPPORTED, "scratch memory for " + std::to_string(n_rows) + " frames cannot be allocated while the stream is captured: call lcrc_reserve first");
+        return fail(c, LCRC_E_UNSUPPORTED, "scratch memory for " + std::to_string(n_rows) +
+                    " frames cannot be allocated while the stream is captured: call lcrc_reserve first");
     const auto drop = [&](void *p) {
         if (p && c->scratch_in_graph) c->allocs.push_back(p);
         else if (p) (void)hipFree(p);            // (waits for launches that still use it)
@@ -520,7 +521,7 @@ int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s)
         (void)hipGetLastError();
         return false;
     };
-    const std::string none = "cannot allocate scratch memory for " + std::to_string(n_rows) + " frames";
+    const auto none = [&] { return fail(c, LCRC_E_NOMEM, "cannot allocate scratch memory for " + std::to_string(n_rows) + " frames"); };
     if (more_rows) {
         const size_t cap = n_rows + n_rows / 4 + 64, Km = c->nets[2].n_inp;
         drop(c->d_feat);
@@ -530,11 +531,11 @@ int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s)
         const size_t feat = c->system == SYS_1BT_DCT ? cap * Km
                             : c->system == SYS_LCRC_GEN ? cap * 2 * (size_t)c->band_nets[0].n_inp
                                                         : cap * (size_t)c->trap_bands * c->trap_len;
-        if (!get((void **)&c->d_feat, feat * sizeof(float))) return fail(c, LCRC_E_NOMEM, none);
+        if (!get((void **)&c->d_feat, feat * sizeof(float))) return none();
         if (c->system != SYS_1BT_DCT && !get((void **)&c->d_minp, cap * Km * sizeof(float))) {
             (void)hipFree(c->d_feat);
             c->d_feat = nullptr;
-            return fail(c, LCRC_E_NOMEM, none);
+            return none();
         }
         c->cap_feat_rows = cap;
     }
@@ -542,7 +543,7 @@ int ensure_traps_scratch(lcrc_ctx *c, size_t n_rows, hipStream_t s)
         drop(c->d_fp8);
         c->d_fp8 = nullptr;
         c->cap_fp8 = 0;
-        if (!get((void **)&c->d_fp8, fp8 + fp8 / 4)) return fail(c, LCRC_E_NOMEM, none);
+        if (!get((void **)&c->d_fp8, fp8 + fp8 / 4)) return none();
         c->cap_fp8 = fp8 + fp8 / 4;
     }
     if (captured) c->scratch_in_graph = true;
